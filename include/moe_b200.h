@@ -467,6 +467,41 @@ int moe_grouped_topk(const void* gating_output, int logits_dtype, int64_t num_to
                      float* topk_weights, int32_t* topk_ids, void* stream);
 
 /*
+ * Balanced routing: experts chosen by score plus a per-expert bias that
+ * steers the load, weighted by the unbiased scores. No reference counterpart.
+ *   s_e = sigmoid(l_e) (scoring_func 1), or the softmax of the row (0)
+ *   c_e = s_e + expert_bias[e]        (expert_bias f32, NULL: no bias)
+ * The experts form num_expert_group equal groups of value the sum of their
+ * two largest c (group_score 1) or their largest c (0); the topk_group best
+ * groups are kept and the top_k experts of largest c among them chosen, in
+ * descending order. Comparisons are those of 64-bit arithmetic; ties go to
+ * the lower index. A NaN c ranks last; ids are always in [0, num_experts).
+ * topk_weights[t, j] (F32/F16/BF16) = s of the j-th chosen, divided by the
+ * sum over the chosen when renormalize (0 when all of them vanish), times
+ * routed_scaling_factor. topk_ids I32 or I64. expert_load (int32
+ * [num_experts], may be NULL): the number of tokens that chose each expert
+ * is ADDED to it. Logits F32/F16/BF16; num_experts <= 1024,
+ * num_expert_group <= 32, top_k <= min(32, topk_group * experts per group).
+ */
+int moe_balanced_topk(const void* router_logits, int logits_dtype, const float* expert_bias,
+                      int64_t num_tokens, int num_experts, int top_k, int renormalize,
+                      int num_expert_group, int topk_group, int group_score, int scoring_func,
+                      float routed_scaling_factor, void* topk_weights, int weights_dtype,
+                      void* topk_ids, int ids_dtype, int32_t* expert_load, void* stream);
+
+/*
+ * Gradient of moe_balanced_topk's weights with respect to the logits: the
+ * chosen ids are constants and the bias has no gradient. grad_weights f32
+ * [num_tokens, top_k]; grad_logits [num_tokens, num_experts] in the logits'
+ * dtype, 16-byte aligned, every element written. An id outside
+ * [0, num_experts) contributes nothing. The ids of a row are distinct.
+ */
+int moe_balanced_topk_backward(const void* router_logits, int logits_dtype, const void* topk_ids,
+                               int ids_dtype, const float* grad_weights, int64_t num_tokens,
+                               int num_experts, int top_k, int renormalize, int scoring_func,
+                               float routed_scaling_factor, void* grad_logits, void* stream);
+
+/*
  * Expert-parallel dispatch plan for this rank's routing (experts sharded in
  * contiguous blocks of num_experts / world per rank). For flat slot r with
  * expert id e = topk_ids[r] and destination rank d = e / (num_experts/world):

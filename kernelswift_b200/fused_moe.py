@@ -154,6 +154,90 @@ def grouped_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor, topk:
     return w, ids
 
 
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 0, "top2": 1}
+
+
+class _BalancedTopK(torch.autograd.Function):
+    """moe_balanced_topk with moe_balanced_topk_backward as its gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, topk, renormalize, groups, kept, scoring, group_score, scale,
+                load, weights_dtype, ids_dtype):
+        T, E = logits.shape
+        dev = logits.device
+        w = torch.empty(T, topk, dtype=weights_dtype, device=dev)
+        ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
+        with torch.cuda.device(dev):
+            _lib.call("moe_balanced_topk", _ptr(logits), _code(logits), _ptr(bias), T, E, topk,
+                      renormalize, groups, kept, group_score, scoring, scale, _ptr(w), _code(w),
+                      _ptr(ids), _code(ids), _ptr(load), _stream(dev))
+        ctx.args = (topk, renormalize, scoring, scale)
+        ctx.save_for_backward(logits, ids)
+        ctx.mark_non_differentiable(ids)
+        return w, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_w, _grad_ids):
+        logits, ids = ctx.saved_tensors
+        topk, renormalize, scoring, scale = ctx.args
+        T, E = logits.shape
+        grad_w = grad_w.to(torch.float32).contiguous()
+        grad = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+        with torch.cuda.device(logits.device):
+            _lib.call("moe_balanced_topk_backward", _ptr(logits), _code(logits), _ptr(ids),
+                      _code(ids), _ptr(grad_w), T, E, topk, renormalize, scoring, scale,
+                      _ptr(grad), _stream(logits.device))
+        return (grad,) + (None,) * 11
+
+
+def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
+                  expert_bias: torch.Tensor | None, topk: int, renormalize: bool = True,
+                  num_expert_group: int = 1, topk_group: int = 1,
+                  scoring_func: str = "sigmoid", group_score: str = "top2",
+                  routed_scaling_factor: float = 1.0,
+                  expert_load: torch.Tensor | None = None,
+                  weights_dtype: torch.dtype = torch.float32,
+                  ids_dtype: torch.dtype = torch.int32) -> tuple[torch.Tensor, torch.Tensor]:
+    """Routing with a balancing bias, in one kernel (moe_balanced_topk).
+
+    Experts are chosen by c = score + expert_bias (fp32 [E], or None), score =
+    sigmoid or softmax of `gating_output` [T, E] (f32/f16/bf16): the
+    `topk_group` of the `num_expert_group` groups with the largest value (the
+    sum of a group's two largest c, or its largest with group_score "max"),
+    then the `topk` largest c among their experts, descending, ties to the
+    lower index; c is compared as in 64-bit arithmetic. The weights are the
+    unbiased scores of the chosen, renormalised over them when asked (0 when
+    they all vanish) and scaled. Returns (topk_weights [T, k], topk_ids [T, k]).
+
+    expert_load: int32 [E]; the number of tokens that chose each expert is
+    added to it (what a training loop adjusts the bias by).
+
+    The weights are differentiable with respect to `gating_output`; the
+    choice and the bias have no gradient.
+    """
+    _check_cuda("gating_output", gating_output)
+    if gating_output.dim() != 2 or gating_output.shape[0] != hidden_states.shape[0]:
+        raise ValueError("gating_output must be [T, E] with T = hidden_states.shape[0]")
+    if scoring_func not in _SCORING:
+        raise ValueError(f"Unsupported scoring_func: {scoring_func}")
+    if group_score not in _GROUP_SCORE:
+        raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORE)}")
+    E, dev = gating_output.shape[1], gating_output.device
+    for name, t, dtype in (("expert_bias", expert_bias, torch.float32),
+                           ("expert_load", expert_load, torch.int32)):
+        if t is not None and (t.dtype != dtype or t.shape != (E,) or t.device != dev):
+            raise ValueError(f"{name} must be a {dtype} [E] = [{E}] tensor on {dev}")
+    if expert_load is not None and not expert_load.is_contiguous():
+        raise ValueError("expert_load must be contiguous (it is added to in place)")
+    bias = None if expert_bias is None else _contig(expert_bias.detach())
+    return _BalancedTopK.apply(_contig(gating_output), bias, topk, int(renormalize),
+                               num_expert_group, topk_group, _SCORING[scoring_func],
+                               _GROUP_SCORE[group_score], float(routed_scaling_factor),
+                               expert_load, weights_dtype, ids_dtype)
+
+
 # ---------------------------------------------------------------------------
 # moe_align_block_size
 # ---------------------------------------------------------------------------

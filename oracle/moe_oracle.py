@@ -81,6 +81,41 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
 # moe_align_block_size (canonical specification)
 # ---------------------------------------------------------------------------
 
+def balanced_topk(logits, bias, topk: int, renormalize: bool = True, num_expert_group: int = 1,
+                  topk_group: int = 1, scoring_func: str = "sigmoid", group_score: str = "top2",
+                  scale: float = 1.0):
+    """Routing by score plus bias, in fp64, row by row: the experts of the
+    best groups in descending order of c = score + bias, ties to the lower
+    index; weights from the unbiased scores (0 when the chosen ones vanish).
+    Returns (weights fp64 [T, k], ids int64 [T, k])."""
+    l = logits.double()
+    T, E = l.shape
+    per = E // num_expert_group
+    if scoring_func == "sigmoid":
+        s = torch.sigmoid(l)
+    else:
+        s = torch.softmax(l, dim=-1)
+        s = torch.where((l == -torch.inf).all(1, keepdim=True), torch.zeros_like(s), s)
+    c = s if bias is None else s + bias.double()
+    c = torch.where(c.isnan(), torch.full_like(c, -torch.inf), c)
+    ids = torch.empty(T, topk, dtype=torch.int64)
+    for t in range(T):
+        row = c[t].tolist()
+        values = []
+        for g in range(num_expert_group):
+            best = sorted(row[g * per:(g + 1) * per], reverse=True)
+            v = sum(best[:2]) if group_score == "top2" else best[0]
+            values.append(v if v == v else -float("inf"))
+        kept = sorted(range(num_expert_group), key=lambda g: (-values[g], g))[:topk_group]
+        pool = [e for e in range(E) if e // per in kept]
+        ids[t] = torch.tensor(sorted(pool, key=lambda e: (-row[e], e))[:topk])
+    w = s.gather(1, ids)
+    if renormalize:
+        total = w.sum(-1, keepdim=True)
+        w = torch.where(total == 0, torch.zeros_like(w), w / total)
+    return w * scale, ids
+
+
 def align_buffer_len(numel: int, num_experts: int, block_m: int) -> int:
     n = numel + num_experts * (block_m - 1)
     return -(-n // block_m) * block_m

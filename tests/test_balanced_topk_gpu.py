@@ -1,0 +1,268 @@
+"""GPU: balanced routing (moe_balanced_topk and its backward) against the fp64
+restatement of the oracle.
+
+Weights: each is off by at most 2 ulp of an exponential, the roundings of a
+sum of up to 1024 terms by lane and tree (37), of the logit's difference to
+the maximum (|l - max| < 16 here) and of two divisions and a product, under
+64 roundings of 2^-24 in all."""
+import pytest
+import torch
+
+from kernelswift_b200 import fused_moe as fm
+from oracle import moe_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+RTOL = 64 * 2.0 ** -24
+STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+SHAPES = [
+    # T, E, k, groups, kept
+    (1, 256, 8, 8, 4),
+    (5, 1, 1, 1, 1),
+    (33, 8, 2, 1, 1),
+    (64, 40, 6, 5, 2),
+    (77, 96, 32, 3, 2),
+    (130, 128, 8, 1, 1),
+    (9, 30, 3, 30, 7),    # groups of one expert
+    (19, 32, 4, 32, 5),
+    (50, 160, 6, 8, 3),   # experts per group not a power of two
+    (21, 384, 8, 1, 1),
+    (700, 64, 6, 4, 4),   # several tokens per block
+    (13, 1000, 16, 20, 9),
+    (7, 1024, 32, 2, 1),
+]
+
+
+def inputs(T, E, dtype, seed, spread=0.2):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(T, E, generator=g) * 1.5).to(dtype)
+    return logits, spread * torch.randn(E, generator=g)
+
+
+def check(logits, bias, w, ids, k, **kw):
+    rw, rids = orc.balanced_topk(logits, bias, k, **kw)
+    assert torch.equal(ids.cpu().long(), rids)
+    torch.testing.assert_close(w.double().cpu(), rw, rtol=RTOL, atol=1e-30)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T,E,k,G,kept", SHAPES)
+def test_matches_fp64(cuda_device, T, E, k, G, kept, score):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        logits, bias = inputs(T, E, dtype, T + E, 0.2 if score == "sigmoid" else 1.0 / E)
+        for group_score, b, renorm in (("top2", bias, True), ("max", bias, False),
+                                       ("top2", None, True)):
+            kw = dict(renormalize=renorm, num_expert_group=G, topk_group=kept,
+                      scoring_func=score, group_score=group_score)
+            x = logits.to(cuda_device)
+            w, ids = fm.balanced_topk(x, x, None if b is None else b.to(cuda_device), k,
+                                      routed_scaling_factor=2.5, **kw)
+            assert w.dtype == torch.float32 and ids.dtype == torch.int32
+            check(logits, b, w, ids, k, scale=2.5, **kw)
+
+
+@pytest.mark.parametrize("score,G,kept", [("sigmoid", 1, 1), ("softmax", 1, 1), ("sigmoid", 8, 3),
+                                          ("softmax", 4, 2)])
+def test_order_of_scores_that_32_bits_cannot_tell_apart(cuda_device, score, G, kept):
+    """The bias moves every expert's score to the same number, up to the
+    rounding of the bias: the order is that of differences near 2^-26."""
+    T, E, k = 40, 128, 8
+    g = torch.Generator().manual_seed(11)
+    for t in range(4):
+        row = torch.randn(1, E, generator=g)
+        s = torch.sigmoid(row.double()) if score == "sigmoid" else torch.softmax(row.double(), -1)
+        bias = (0.7 - s[0]).float()
+        logits = row.repeat(T, 1)
+        x = logits.to(cuda_device)
+        kw = dict(num_expert_group=G, topk_group=kept, scoring_func=score)
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, **kw)
+        check(logits, bias, w, ids, k, **kw)
+
+
+def test_true_ties_go_to_the_lower_index(cuda_device):
+    x = torch.zeros(3, 64, device=cuda_device)
+    x[1, 40] = 1.0
+    x[2] = -50.0
+    _, ids = fm.balanced_topk(x, x, None, 3)
+    assert ids.tolist() == [[0, 1, 2], [40, 0, 1], [0, 1, 2]]
+    _, ids = fm.balanced_topk(x, x, None, 3, num_expert_group=4, topk_group=2)
+    assert ids.tolist() == [[0, 1, 2], [40, 0, 1], [0, 1, 2]]
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("G,kept", [(1, 1), (4, 2)])
+def test_masked_experts_and_empty_rows(cuda_device, score, G, kept):
+    """Logits of -inf and of the type's lowest value, biases of -inf, rows
+    with nothing left: the ids stay valid, and as the definition says."""
+    T, E, k = 6, 32, 4
+    logits, bias = inputs(T, E, torch.float32, 3)
+    logits[0, ::2] = -torch.inf
+    logits[1] = -torch.inf
+    logits[2, 1:] = torch.finfo(torch.float32).min
+    logits[3, 5] = 60.0
+    bias[7] = -torch.inf
+    bias[9:30] = -torch.inf
+    x = logits.to(cuda_device)
+    for renorm in (True, False):
+        kw = dict(renormalize=renorm, num_expert_group=G, topk_group=kept, scoring_func=score)
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, **kw)
+        rw, rids = orc.balanced_topk(logits, bias, k, **kw)
+        assert torch.equal(ids.cpu().long(), rids)
+        # scores below fp32's range vanish; a row of them has no weights
+        rw = torch.where(rw < 1e-37, torch.zeros_like(rw), rw)
+        got = torch.where(w.cpu().double() < 1e-37, torch.zeros_like(rw), w.cpu().double())
+        far = (logits.gather(1, rids) < -87).all(1)  # chosen scores under 2^-126
+        torch.testing.assert_close(got[~far], rw[~far], rtol=RTOL, atol=1e-30)
+        assert torch.isfinite(w).all()
+
+
+def test_nan_ranks_last_and_ids_stay_valid(cuda_device):
+    x = torch.randn(4, 16, device=cuda_device)
+    x[0, 3] = torch.nan
+    x[1] = torch.nan
+    w, ids = fm.balanced_topk(x, x, None, 4)
+    assert ((ids >= 0) & (ids < 16)).all() and 3 not in ids[0].tolist()
+    assert ids[1].tolist() == [0, 1, 2, 3] and w[1].isnan().all()
+    assert torch.isfinite(w[[0, 2, 3]]).all()
+    w, ids = fm.balanced_topk(x, x, None, 4, scoring_func="softmax", renormalize=False)
+    assert ((ids >= 0) & (ids < 16)).all() and w[:2].isnan().all()
+
+
+def test_load_is_added_and_types_are_kept(cuda_device):
+    T, E, k = 501, 48, 5
+    logits, bias = inputs(T, E, torch.float32, 8)
+    x = logits.to(cuda_device)
+    load = torch.full((E,), 7, dtype=torch.int32, device=cuda_device)
+    w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, expert_load=load,
+                              weights_dtype=torch.bfloat16, ids_dtype=torch.int64)
+    assert w.dtype == torch.bfloat16 and ids.dtype == torch.int64
+    rw, rids = orc.balanced_topk(logits, bias, k)
+    assert torch.equal(ids.cpu(), rids)
+    torch.testing.assert_close(w.double().cpu(), rw, rtol=2.0 ** -8 + RTOL, atol=0)
+    assert torch.equal(load.cpu().long(), 7 + torch.bincount(rids.reshape(-1), minlength=E))
+
+
+def test_no_tokens_and_views(cuda_device):
+    x = torch.empty(0, 16, device=cuda_device)
+    w, ids = fm.balanced_topk(x, x, None, 2)
+    assert w.shape == (0, 2) and ids.shape == (0, 2)
+    wide = torch.randn(20, 2 * 24, device=cuda_device)
+    for view in (wide[:, 1:25], wide[::2, ::2], wide[:1, :24].expand(20, 24)):
+        w, ids = fm.balanced_topk(view, view, None, 3)
+        check(view.cpu(), None, w, ids, 3)
+
+
+def formula(logits, bias, gw, k, score, renorm, scale, ids):
+    """fp64 gradient by autograd through the definition, ids given."""
+    leaf = logits.double().requires_grad_()
+    s = torch.sigmoid(leaf) if score == "sigmoid" else torch.softmax(leaf, -1)
+    w = s.gather(1, ids)
+    if renorm:
+        w = w / w.sum(-1, keepdim=True)
+    (scale * w * gw.double()).sum().backward()
+    return leaf.grad
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k,G,kept", SHAPES)
+def test_gradient(cuda_device, T, E, k, G, kept, score, renorm):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        logits, bias = inputs(T, E, dtype, 3 * T + E, 0.2 if score == "sigmoid" else 1.0 / E)
+        x = logits.to(cuda_device).requires_grad_()
+        gw = torch.randn(T, k, generator=torch.Generator().manual_seed(1))
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, renormalize=renorm,
+                                  num_expert_group=G, topk_group=kept, scoring_func=score,
+                                  routed_scaling_factor=1.5)
+        assert w.requires_grad and not ids.requires_grad
+        w.backward(gw.to(cuda_device))
+        want = formula(logits, bias, gw, k, score, renorm, 1.5, ids.cpu().long())
+        assert x.grad.dtype == dtype
+        # g_j - mean and the sum over k cancel: the error goes by the row's
+        # largest |g| times the largest score, not by each entry
+        room = RTOL * 1.5 * gw.abs().amax(1, keepdim=True).double() * k
+        err = (x.grad.double().cpu() - want).abs()
+        # an fp16 entry below 2^-14 is subnormal: half a step of 2^-24
+        tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+        assert (err <= room + STEP[dtype] * want.abs() + tiny).all()
+
+
+def test_gradient_against_differences(cuda_device):
+    """(f(l + h) - f(l - h)) / 2h of the fp64 definition at fixed ids."""
+    T, E, k = 3, 24, 4
+    for score in ("sigmoid", "softmax"):
+        for renorm in (True, False):
+            logits, bias = inputs(T, E, torch.float32, 21)
+            x = logits.to(cuda_device).requires_grad_()
+            w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, renormalize=renorm,
+                                      scoring_func=score)
+            gw = torch.linspace(-1, 2, T * k).view(T, k)
+            (w * gw.to(cuda_device)).sum().backward()
+            idx = ids.cpu().long()
+
+            def f(l):
+                s = torch.sigmoid(l) if score == "sigmoid" else torch.softmax(l, -1)
+                v = s.gather(1, idx)
+                v = v / v.sum(-1, keepdim=True) if renorm else v
+                return (v * gw.double()).sum()
+
+            h, base = 1e-5, logits.double()
+            for t in range(T):
+                for e in range(E):
+                    d = torch.zeros(T, E, dtype=torch.float64)
+                    d[t, e] = h
+                    diff = (f(base + d) - f(base - d)) / (2 * h)
+                    # differences: h^2 / 6 of a third derivative under 10, and
+                    # 2^-53 / h of rounding; the kernel: as in test_gradient
+                    assert abs(x.grad[t, e].item() - diff.item()) < 1e-9 + 8 * RTOL
+
+
+def test_gradient_of_expanded_logits(cuda_device):
+    row = torch.randn(1, 16, device=cuda_device, requires_grad=True)
+    x = row.expand(6, 16)
+    w, ids = fm.balanced_topk(x, x, None, 3, renormalize=False)
+    w.sum().backward()
+    want = formula(row.detach().cpu(), None, torch.full((1, 3), 6.0), 3, "sigmoid", False, 1.0,
+                   ids[:1].cpu().long())
+    # six equal terms: five more roundings
+    torch.testing.assert_close(row.grad.double().cpu(), want, rtol=2 * RTOL, atol=1e-30)
+
+
+def test_captured_and_on_another_stream(cuda_device):
+    T, E, k = 16, 256, 8
+    logits, bias = inputs(T, E, torch.float32, 5)
+    b = bias.to(cuda_device)
+    static = torch.zeros(T, E, device=cuda_device)
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        fm.balanced_topk(static, static, b, k, num_expert_group=8, topk_group=4)
+        w, ids = fm.balanced_topk(logits.to(cuda_device), static, b, k)
+    torch.cuda.current_stream(cuda_device).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w, ids = fm.balanced_topk(static, static, b, k, num_expert_group=8, topk_group=4)
+    for seed in (1, 2):
+        logits, _ = inputs(T, E, torch.float32, seed)
+        static.copy_(logits)
+        graph.replay()
+        check(logits, bias, w, ids, k, num_expert_group=8, topk_group=4)
+
+
+def test_refusals(cuda_device):
+    from kernelswift_b200._lib import MoeError
+
+    x = torch.randn(4, 32, device=cuda_device)
+    with pytest.raises(MoeError):
+        fm.balanced_topk(x, x, None, 9, num_expert_group=4, topk_group=1)
+    with pytest.raises(MoeError):
+        fm.balanced_topk(x, x, None, 33)
+    with pytest.raises(MoeError):
+        fm.balanced_topk(x, x, None, 2, num_expert_group=5)
+    with pytest.raises(ValueError):
+        fm.balanced_topk(x, x, torch.zeros(31, device=cuda_device), 2)
+    with pytest.raises(ValueError):
+        fm.balanced_topk(x, x, torch.zeros(32), 2)
+    with pytest.raises(ValueError):
+        fm.balanced_topk(x, x, None, 2, expert_load=torch.zeros(32, device=cuda_device))
