@@ -501,6 +501,59 @@ int moe_balanced_topk_backward(const void* router_logits, int logits_dtype, cons
                                int num_experts, int top_k, int renormalize, int scoring_func,
                                float routed_scaling_factor, void* grad_logits, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Dense block-scaled fp8: quantisers and product (the layer's shared expert, */
+/* or any linear layer on e4m3 weights). No reference counterpart.           */
+/*                                                                          */
+/* e4m3 matrices are row-major with rows that start on 16-byte boundaries    */
+/* (base pointer and row stride multiples of 16; any number of columns).     */
+/* scale_format 0: fp32 scales, 1: UE8M0 bytes b meaning 2^(b - 127).        */
+/* Strides are in elements.                                                  */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Quantises rows [num_rows, cols] (F32/F16/BF16) to e4m3 with one scale per
+ * row and 128 columns. gated: the input row is [gate | up], 2 * cols wide,
+ * and silu(gate) * up is quantised. fp32: scale = absmax / 448 (1 for an
+ * all-zero group), q = the e4m3 nearest to x * 448 / absmax. UE8M0: the least
+ * power of two with absmax / scale <= 448, q nearest to x / scale. A NaN stays
+ * a NaN and does not count for absmax; a group that holds an infinity has an
+ * infinite scale (fp32), or saturates there (UE8M0). The scale of row t,
+ * block kb goes to scale[t * scale_row_stride + kb * scale_block_stride].
+ */
+int moe_fp8_quantize_rows(const void* x, int x_dtype, int64_t num_rows, int64_t cols,
+                          int64_t ld_x, int gated, int scale_format, void* q, int64_t ld_q,
+                          void* scale, int64_t scale_row_stride, int64_t scale_block_stride,
+                          void* stream);
+
+/* The same with one scale per 128 x 128 block (weights): scale
+ * [ceil(rows / 128), ceil(cols / 128)] dense. */
+int moe_fp8_quantize_blocks(const void* w, int w_dtype, int64_t rows, int64_t cols, int64_t ld_w,
+                            int scale_format, void* q, int64_t ld_q, void* scale, void* stream);
+
+/*
+ * out[t, n] = addend[t, n] + sum_kb x_scale[t, kb] * w_scale[n / 128, kb] *
+ *             sum_{k in block kb} x[t, k] * w[n, k]
+ * x [num_rows, inner] and w [out_cols, inner] e4m3; x_scale addressed by its
+ * two strides, w_scale dense [ceil(out_cols / 128), ceil(inner / 128)];
+ * addend (may be NULL) and out in out_dtype (F32/F16/BF16), out may be the
+ * addend. Products run on the tensor cores and are summed in fp32; with fp32
+ * scales each 128-wide block's product is scaled and added in fp32 registers,
+ * with UE8M0 the tensor core scales. A row's result does not depend on the
+ * other rows' values. `status` as for moe_fused_experts (may be NULL).
+ */
+int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale, int64_t xs_row_stride,
+                   int64_t xs_block_stride, const void* w, int64_t ld_w, const void* w_scale,
+                   int scale_format, int64_t num_rows, int64_t out_cols, int64_t inner,
+                   const void* addend, int64_t ld_addend, void* out, int64_t ld_out,
+                   int out_dtype, int32_t* status, void* stream);
+
+/* How moe_fp8_matmul runs these sizes (no GPU needed, for 148 SMs): info[0]
+ * 1 when tokens lie on the MMA's rows (0: the weights do), [1] columns per
+ * tile, [2] CTAs that split K, [3] CTAs launched. */
+int moe_fp8_matmul_plan(int64_t num_rows, int64_t out_cols, int64_t inner, int scale_format,
+                        int32_t* info);
+
 /*
  * Expert-parallel dispatch plan for this rank's routing (experts sharded in
  * contiguous blocks of num_experts / world per rank). For flat slot r with

@@ -106,6 +106,12 @@ SIGNATURES = {
                                  ctypes.c_float, _vp, _int, _vp, _int, _vp, _vp]),
     "moe_balanced_topk_backward": (_int, [_vp, _int, _vp, _int, _vp, _i64, _int, _int, _int,
                                           _int, ctypes.c_float, _vp, _vp]),
+    "moe_fp8_quantize_rows": (_int, [_vp, _int, _i64, _i64, _i64, _int, _int, _vp, _i64, _vp,
+                                     _i64, _i64, _vp]),
+    "moe_fp8_quantize_blocks": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp]),
+    "moe_fp8_matmul": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64,
+                              _vp, _i64, _vp, _i64, _int, _vp, _vp]),
+    "moe_fp8_matmul_plan": (_int, [_i64, _i64, _i64, _int, _vp]),
     "moe_combine_rows": (_int, [_vp, _int, _vp, _vp, _int, _i64, _int, _i64, _vp, _int, _vp]),
     "moe_selftest_wait_timeout": (_int, [_vp, _int, _vp]),
     "moe_selftest_sf_copy": (_int, [_vp, _vp, _vp, _vp]),

@@ -1,0 +1,314 @@
+// Quantisers of the dense block-scaled fp8 product (fp8_matmul.cu).
+//
+// Rows: each group of 128 columns of a row has one scale,
+//   fp32:   s = absmax / 448 (1 for an all-zero group), q = e4m3 nearest to
+//           x * 448 / absmax,
+//   UE8M0:  s = 2^(b - 127), the least power of two with absmax / s <= 448
+//           (b = 127 for an all-zero group), q = e4m3 nearest to x / s.
+// With `gated` the row is silu(gate) * up of an input row [gate | up], so the
+// down product's operand is written straight from the gate-up product.
+// Blocks: the same with one scale for each 128 x 128 block (weights).
+//
+// x * 448 / absmax is computed as (x * 0.875) / (absmax * 2^-9), one IEEE
+// division: for 16-bit inputs numerator and denominator are exact, so a
+// quotient on the midpoint of two e4m3 values is recognised as such (a
+// multiplication by a rounded reciprocal falls to either side of it).
+//
+// What bounds the row kernel: HBM. A half-warp holds a group (8 columns per
+// lane, one 16-byte load for 16-bit inputs), a warp 1024 columns of a row with
+// its four loads in flight before the first is used.
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace ksw {
+namespace {
+
+constexpr int kRowWarps = 8;
+constexpr int kChunk = 1024;  // columns of a row per warp
+constexpr int kIters = kChunk / 256;
+
+struct QuantRows {
+  const void* x;
+  int64_t T, K, ld_x;
+  uint8_t* q;
+  int64_t ld_q;
+  void* scale;
+  int64_t s_row, s_blk;  // strides of the scale, in elements
+};
+
+// Eight consecutive elements from `p`, of which `n` exist (the rest are 0).
+template <typename Tin, bool VEC>
+__device__ __forceinline__ void load8(const Tin* p, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n >= 8) {
+      if constexpr (std::is_same<Tin, float>::value) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const Tin* e = reinterpret_cast<const Tin*>(&a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+}
+
+__device__ __forceinline__ float silu_up(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ double silu_up(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+
+// Two e4m3 bytes, round to nearest even; a NaN stays one, beyond 448 saturates.
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3));
+}
+
+// The factors of x * 448 / amax = (x * num) / den; up keeps den normal.
+struct Ratio {
+  float num, den;
+};
+__device__ __forceinline__ Ratio ratio_of(float amax) {
+  if (!(amax > 0.0f)) return {0.875f, 0.875f};
+  const float up = amax < 0x1p-100f ? 0x1p100f : 1.0f;
+  return {0.875f * up, amax * up * 0x1p-9f};
+}
+__device__ __forceinline__ float fp32_scale(float amax) {
+  return amax > 0.0f ? amax / 448.0f : 1.0f;
+}
+
+template <typename Tin, bool VEC, bool GATED, bool UE8M0>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    fp8_quantize_rows_kernel(const QuantRows p, int chunks) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the warps of a block take neighbouring rows at the same columns, so that
+  // their scales meet in the same sectors
+  const int64_t t = int64_t(blockIdx.x) * kRowWarps + warp;
+  if (t >= p.T) return;
+  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+    const int64_t c0 = int64_t(chunk) * kChunk + 8 * lane;
+    const Tin* row = static_cast<const Tin*>(p.x) + t * p.ld_x;
+    float v[kIters][8];
+    float u[GATED ? kIters : 1][8];
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      const int64_t c = c0 + 256 * i;
+      const int n = int(min(int64_t(8), max(int64_t(0), p.K - c)));
+      load8<Tin, VEC>(row + c, n, v[i]);
+      if constexpr (GATED) load8<Tin, VEC>(row + p.K + c, n, u[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      const int64_t c = c0 + 256 * i;
+      float amax = 0.0f;
+      [[maybe_unused]] float gate[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (GATED) {
+          gate[e] = v[i][e];
+          v[i][e] = silu_up(v[i][e], u[i][e]);
+        }
+        amax = fmaxf(amax, fabsf(v[i][e]));
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1)
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      uint32_t w[4];
+      const int64_t blk = c / 128;
+      const bool writer = (lane & 15) == 0 && c < p.K;
+      if constexpr (UE8M0) {
+        uint32_t b = ue8m0_byte(amax);
+        if constexpr (GATED) {
+          // a maximum within the rounding of the 32-bit silu (under 8 ulp) of
+          // 448 * 2^k decides the scale by its 64-bit value
+          const uint32_t bits = __float_as_uint(amax);
+          const int off = int(bits & 0x7fffffu) - 0x600000;
+          const bool near = amax > 0.0f && amax < INFINITY && off >= -16 && off <= 16;
+          if (__any_sync(0xffffffffu, near)) {
+            double m = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              m = fmax(m, fabs(silu_up(double(gate[e]), double(u[i][e]))));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (near) {
+              const int e = int(bits >> 23);
+              const double border = ldexp(1.75, e - 127);
+              b = uint32_t(min(max(e - 8 + (m > border ? 1 : 0), 0), 254));
+            }
+          }
+        }
+        const float inv = ue8m0_inv_scale(b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
+        if (writer) static_cast<uint8_t*>(p.scale)[t * p.s_row + blk * p.s_blk] = uint8_t(b);
+      } else {
+        const Ratio r = ratio_of(amax);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = e4m3x2(v[i][2 * e] * r.num / r.den, v[i][2 * e + 1] * r.num / r.den);
+        if (writer) static_cast<float*>(p.scale)[t * p.s_row + blk * p.s_blk] = fp32_scale(amax);
+      }
+      // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
+      // 8 bytes at a column below K are inside the row
+      if (c < p.K)
+        *reinterpret_cast<uint2*>(p.q + t * p.ld_q + c) =
+            make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  }
+}
+
+// One block per 128 x 128 block of the matrix: 8 warps of 16 rows, lane l
+// holds columns l, l + 32, ... of each row. One-time work (weights).
+constexpr int kBlkWarps = 8;
+
+template <typename Tin, bool UE8M0>
+__global__ void __launch_bounds__(32 * kBlkWarps)
+    fp8_quantize_blocks_kernel(const Tin* __restrict__ w, int64_t N, int64_t K, int64_t ld_w,
+                               uint8_t* __restrict__ q, int64_t ld_q, void* scale,
+                               int64_t col_blocks) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t nb = blockIdx.x / col_blocks, kb = blockIdx.x % col_blocks;
+  __shared__ float s_max[kBlkWarps];
+  float v[16][4];
+  float amax = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = nb * 128 + warp * 16 + r, k = kb * 128 + lane + 32 * j;
+      v[r][j] = n < N && k < K ? to_f32(w[n * ld_w + k]) : 0.0f;
+      amax = fmaxf(amax, fabsf(v[r][j]));
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) s_max[warp] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBlkWarps; ++i) amax = fmaxf(amax, s_max[i]);
+  Ratio ratio = ratio_of(amax);
+  if constexpr (UE8M0) {
+    const uint32_t b = ue8m0_byte(amax);
+    ratio = {ue8m0_inv_scale(b), 1.0f};
+    if (threadIdx.x == 0) static_cast<uint8_t*>(scale)[blockIdx.x] = uint8_t(b);
+  } else {
+    if (threadIdx.x == 0) static_cast<float*>(scale)[blockIdx.x] = fp32_scale(amax);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = nb * 128 + warp * 16 + r, k = kb * 128 + lane + 32 * j;
+      const float x = v[r][j] * ratio.num;
+      if (n < N && k < K)
+        q[n * ld_q + k] = uint8_t(e4m3x2(UE8M0 ? x : x / ratio.den, 0.0f));
+    }
+}
+
+template <typename Tin, bool VEC, bool GATED>
+int launch_rows(const QuantRows& p, int ue8m0, cudaStream_t s) {
+  const int64_t row_blocks = ceil_div(p.T, kRowWarps);
+  const int chunks = int(ceil_div(p.K, kChunk));
+  const dim3 grid(unsigned(row_blocks), unsigned(std::min(chunks, 65535)));
+  if (ue8m0)
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, true>, grid, dim3(32 * kRowWarps), 0, s,
+               p, chunks);
+  else
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, false>, grid, dim3(32 * kRowWarps), 0, s,
+               p, chunks);
+  return MOE_OK;
+}
+
+template <typename Tin>
+int launch_rows_t(const QuantRows& p, int gated, int ue8m0, cudaStream_t s) {
+  // 16-byte loads when every row, and the up half, starts on such a boundary
+  const bool vec = aligned16(p.x) && (p.ld_x * sizeof(Tin)) % 16 == 0 &&
+                   (!gated || (p.K * sizeof(Tin)) % 16 == 0);
+  if (gated)
+    return vec ? launch_rows<Tin, true, true>(p, ue8m0, s)
+               : launch_rows<Tin, false, true>(p, ue8m0, s);
+  return vec ? launch_rows<Tin, true, false>(p, ue8m0, s)
+             : launch_rows<Tin, false, false>(p, ue8m0, s);
+}
+
+template <typename Tin>
+int launch_blocks(const void* w, int64_t N, int64_t K, int64_t ld_w, int ue8m0, uint8_t* q,
+                  int64_t ld_q, void* scale, cudaStream_t s) {
+  const int64_t kb = ceil_div(K, 128), blocks = ceil_div(N, 128) * kb;
+  if (ue8m0)
+    KSW_LAUNCH(fp8_quantize_blocks_kernel<Tin, true>, dim3(unsigned(blocks)),
+               dim3(32 * kBlkWarps), 0, s, static_cast<const Tin*>(w), N, K, ld_w, q, ld_q, scale,
+               kb);
+  else
+    KSW_LAUNCH(fp8_quantize_blocks_kernel<Tin, false>, dim3(unsigned(blocks)),
+               dim3(32 * kBlkWarps), 0, s, static_cast<const Tin*>(w), N, K, ld_w, q, ld_q, scale,
+               kb);
+  return MOE_OK;
+}
+
+int check_source(const char* what, int dtype, int64_t rows, int64_t cols, int64_t ld,
+                 int64_t wide, int scale_format, const void* q, int64_t ld_q) {
+  const std::string name(what);
+  KSW_REQUIRE(dtype == MOE_DTYPE_F32 || dtype == MOE_DTYPE_F16 || dtype == MOE_DTYPE_BF16,
+              MOE_ERR_INVALID_ARG, name + ": source dtype must be f32/f16/bf16");
+  KSW_REQUIRE(rows >= 0 && cols >= 1, MOE_ERR_INVALID_ARG, name + ": bad sizes");
+  KSW_REQUIRE(rows <= (int64_t(1) << 31) - 8 && cols <= (int64_t(1) << 31) - 8,
+              MOE_ERR_UNSUPPORTED, name + ": sizes beyond 2^31");
+  KSW_REQUIRE(ld >= wide, MOE_ERR_INVALID_ARG, name + ": row stride shorter than a row");
+  KSW_REQUIRE(scale_format == 0 || scale_format == 1, MOE_ERR_INVALID_ARG,
+              name + ": scale_format must be 0 (fp32) or 1 (UE8M0)");
+  KSW_REQUIRE(aligned16(q) && ld_q % 16 == 0 && ld_q >= round_up(cols, 16), MOE_ERR_INVALID_ARG,
+              name + ": the fp8 rows must start on 16-byte boundaries");
+  return MOE_OK;
+}
+
+}  // namespace
+}  // namespace ksw
+
+extern "C" int moe_fp8_quantize_rows(const void* x, int x_dtype, int64_t num_rows, int64_t cols,
+                                     int64_t ld_x, int gated, int scale_format, void* q,
+                                     int64_t ld_q, void* scale, int64_t scale_row_stride,
+                                     int64_t scale_block_stride, void* stream) {
+  using namespace ksw;
+  int st = check_source("fp8_quantize_rows", x_dtype, num_rows, cols, ld_x,
+                        gated ? 2 * cols : cols, scale_format, q, ld_q);
+  if (st != MOE_OK) return st;
+  if ((st = check_device(nullptr)) != MOE_OK) return st;
+  if (num_rows == 0) return MOE_OK;
+  KSW_REQUIRE(x && q && scale, MOE_ERR_INVALID_ARG, "fp8_quantize_rows: null pointer");
+  const QuantRows p = {x,    num_rows,         cols, ld_x, static_cast<uint8_t*>(q), ld_q, scale,
+                       scale_row_stride, scale_block_stride};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x_dtype == MOE_DTYPE_F32) return launch_rows_t<float>(p, gated, scale_format, s);
+  if (x_dtype == MOE_DTYPE_BF16) return launch_rows_t<__nv_bfloat16>(p, gated, scale_format, s);
+  return launch_rows_t<__half>(p, gated, scale_format, s);
+}
+
+extern "C" int moe_fp8_quantize_blocks(const void* w, int w_dtype, int64_t rows, int64_t cols,
+                                       int64_t ld_w, int scale_format, void* q, int64_t ld_q,
+                                       void* scale, void* stream) {
+  using namespace ksw;
+  int st = check_source("fp8_quantize_blocks", w_dtype, rows, cols, ld_w, cols, scale_format, q,
+                        ld_q);
+  if (st != MOE_OK) return st;
+  KSW_REQUIRE(ceil_div(rows, 128) * ceil_div(cols, 128) < (int64_t(1) << 31),
+              MOE_ERR_UNSUPPORTED, "fp8_quantize_blocks: too many blocks");
+  if ((st = check_device(nullptr)) != MOE_OK) return st;
+  if (rows == 0) return MOE_OK;
+  KSW_REQUIRE(w && q && scale, MOE_ERR_INVALID_ARG, "fp8_quantize_blocks: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* qb = static_cast<uint8_t*>(q);
+  if (w_dtype == MOE_DTYPE_F32)
+    return launch_blocks<float>(w, rows, cols, ld_w, scale_format, qb, ld_q, scale, s);
+  if (w_dtype == MOE_DTYPE_BF16)
+    return launch_blocks<__nv_bfloat16>(w, rows, cols, ld_w, scale_format, qb, ld_q, scale, s);
+  return launch_blocks<__half>(w, rows, cols, ld_w, scale_format, qb, ld_q, scale, s);
+}

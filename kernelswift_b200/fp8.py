@@ -1,0 +1,192 @@
+"""Dense block-scaled fp8 for the layers around the routed experts: the
+quantisers, the product of e4m3 matrices with one scale per 128 columns of a
+row and per 128x128 block of the weights, and the SwiGLU MLP that chains them
+(the shared expert of an MoE layer).
+
+Formats: scale_format "fp32" (scale = absmax / 448) or "ue8m0" (uint8 bytes b
+meaning the power of two 2^(b - 127), applied by the tensor core). A scale
+tensor's dtype says which it is. The grouped GEMMs of fused_moe take the same
+formats per expert.
+
+Everything runs in libmoe_b200.so on the current stream of the operands'
+device; nothing allocates but the outputs, and a call can be captured in a
+CUDA graph. There is no CPU path and no gradient: these are serving operators.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .fused_moe import _check_cuda, _code, _contig, _DTYPE_CODE, _ptr, _stream
+
+_FORMAT = {"fp32": 0, "ue8m0": 1}
+_SCALE_FORMAT = {torch.float32: 0, torch.uint8: 1}
+_FLOAT = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _round_up(n: int, m: int) -> int:
+    return -(-n // m) * m
+
+
+def _no_grad_needed(name: str, t: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(f"{name} requires a gradient; the fp8 operators have none "
+                         "(call them under torch.no_grad())")
+
+
+def _rows_of(name: str, t: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor whose rows are dense: `t`, or a dense copy."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.numel() == 0:
+        return t
+    return t.contiguous()
+
+
+def _fp8_rows(name: str, t: torch.Tensor) -> torch.Tensor:
+    """An e4m3 matrix whose rows start on 16-byte boundaries: `t`, or a copy
+    with its row pitch padded."""
+    if t.dtype != torch.float8_e4m3fn or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D float8_e4m3fn tensor")
+    rows, cols = t.shape
+    if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= cols
+            and t.data_ptr() % 16 == 0):
+        return t
+    q = torch.empty(rows, _round_up(cols, 16), dtype=t.dtype, device=t.device)
+    q[:, :cols].view(torch.uint8).copy_(t.view(torch.uint8))
+    return q[:, :cols]
+
+
+def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = False
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantises x [T, K] (f32/f16/bf16) to e4m3 with one scale per row and
+    128 columns (moe_fp8_quantize_rows). gated: x is [T, 2K], gate then up, and
+    silu(gate) * up [T, K] is quantised. Returns (q float8_e4m3fn [T, K], scale
+    [T, ceil(K / 128)], float32 or uint8), the operands of block_matmul: views
+    whose row pitch is padded to 16 bytes (q) and 4 (scale bytes); fp32 scales
+    lie column by column."""
+    _check_cuda("x", x)
+    _no_grad_needed("x", x)
+    if scale_format not in _FORMAT:
+        raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
+    if x.dim() != 2 or x.dtype not in _FLOAT or (gated and x.shape[1] % 2):
+        raise ValueError("x must be a 2-D f32/f16/bf16 tensor, of an even width when gated")
+    x = _rows_of("x", x)
+    T = x.shape[0]
+    K = x.shape[1] // 2 if gated else x.shape[1]
+    if K < 1:
+        raise ValueError("x has no columns")
+    dev, kb = x.device, -(-K // 128)
+    q = torch.empty(T, _round_up(K, 16), dtype=torch.float8_e4m3fn, device=dev)
+    if scale_format == "fp32":
+        scale = torch.empty(kb, _round_up(T, 4), dtype=torch.float32, device=dev).t()[:T]
+    else:
+        scale = torch.empty(T, _round_up(kb, 4), dtype=torch.uint8, device=dev)[:, :kb]
+    with torch.cuda.device(dev):
+        _lib.call("moe_fp8_quantize_rows", _ptr(x), _code(x), T, K, max(x.stride(0), x.shape[1]),
+                  int(gated), _FORMAT[scale_format], _ptr(q), q.stride(0), _ptr(scale),
+                  scale.stride(0), scale.stride(1), _stream(dev))
+    return q[:, :K], scale
+
+
+def quantize_blocks(w: torch.Tensor, scale_format: str = "ue8m0"
+                    ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantises weights w [N, K] (f32/f16/bf16) to e4m3 with one scale per
+    128x128 block (moe_fp8_quantize_blocks), once per weight version. Returns
+    (q float8_e4m3fn [N, K] of a row pitch padded to 16 bytes, scale
+    [ceil(N / 128), ceil(K / 128)], float32 or uint8)."""
+    _check_cuda("w", w)
+    if scale_format not in _FORMAT:
+        raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
+    if w.dim() != 2 or w.dtype not in _FLOAT or w.numel() == 0:
+        raise ValueError("w must be a 2-D f32/f16/bf16 tensor")
+    w = _rows_of("w", w.detach())
+    N, K = w.shape
+    dev = w.device
+    q = torch.empty(N, _round_up(K, 16), dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(-(-N // 128), -(-K // 128), device=dev,
+                        dtype=torch.float32 if scale_format == "fp32" else torch.uint8)
+    with torch.cuda.device(dev):
+        _lib.call("moe_fp8_quantize_blocks", _ptr(w), _code(w), N, K, max(w.stride(0), K),
+                  _FORMAT[scale_format], _ptr(q), q.stride(0), _ptr(scale), _stream(dev))
+    return q[:, :K], scale
+
+
+def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                 out_dtype: torch.dtype = torch.bfloat16, addend: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, status: torch.Tensor | None = None
+                 ) -> torch.Tensor:
+    """out [T, N] = x w^T (+ addend) for block-scaled e4m3 operands
+    (moe_fp8_matmul).
+
+    x float8_e4m3fn [T, K] with x_scale [T, ceil(K / 128)], w [N, K] with
+    w_scale [ceil(N / 128), ceil(K / 128)]; both scales float32 or both uint8
+    (UE8M0). Rows that do not start on 16-byte boundaries are copied first
+    (quantize_rows and quantize_blocks pad them). addend [T, N] has out's
+    dtype and may be out itself. Summed in fp32, rounded once to out_dtype
+    (bf16, f16 or f32). status: optional int32 device word (moe_read_status).
+    """
+    for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
+        _check_cuda(name, t)
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    x, w = _fp8_rows("x", x), _fp8_rows("w", w)
+    (T, K), N = x.shape, w.shape[0]
+    kb = -(-K // 128)
+    if w.shape[1] != K or K < 1 or N < 1:
+        raise ValueError(f"w {tuple(w.shape)} does not match x {tuple(x.shape)}")
+    if x_scale.dtype not in _SCALE_FORMAT or w_scale.dtype != x_scale.dtype:
+        raise ValueError("x_scale and w_scale must both be float32 or both uint8 (UE8M0)")
+    if x_scale.shape != (T, kb) or w_scale.shape != (-(-N // 128), kb):
+        raise ValueError(f"scales must be [T, {kb}] and [{-(-N // 128)}, {kb}], got "
+                         f"{tuple(x_scale.shape)} and {tuple(w_scale.shape)}")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in _FLOAT:
+        raise ValueError("out_dtype must be bf16, f16 or f32")
+    dev = x.device
+    if out is None:
+        out = torch.empty(T, N, dtype=out_dtype, device=dev)
+    elif (out.shape != (T, N) or out.device != dev or out.stride(1) != 1
+          or out.stride(0) < N and T > 1):
+        raise ValueError(f"out must be a [{T}, {N}] tensor with dense rows on {dev}")
+    if addend is not None:
+        _no_grad_needed("addend", addend)
+        if addend.shape != (T, N) or addend.dtype != out_dtype or addend.device != dev:
+            raise ValueError(f"addend must be a {out_dtype} [{T}, {N}] tensor on {dev}")
+        addend = _rows_of("addend", addend)
+    w_scale = w_scale if w_scale.is_contiguous() else w_scale.contiguous()
+    with torch.cuda.device(dev):
+        _lib.call("moe_fp8_matmul", _ptr(x), max(x.stride(0), _round_up(K, 16)), _ptr(x_scale),
+                  x_scale.stride(0), x_scale.stride(1), _ptr(w), max(w.stride(0), _round_up(K, 16)),
+                  _ptr(w_scale), _SCALE_FORMAT[x_scale.dtype], T, N, K, _ptr(addend),
+                  0 if addend is None else max(addend.stride(0), N), _ptr(out),
+                  max(out.stride(0), N), _DTYPE_CODE[out_dtype], _ptr(status), _stream(dev))
+    return out
+
+
+def block_matmul_plan(num_rows: int, out_cols: int, inner: int, scale_format: str = "ue8m0"
+                      ) -> dict:
+    """How block_matmul runs these sizes (moe_fp8_matmul_plan; no GPU needed)."""
+    import ctypes
+
+    info = (ctypes.c_int32 * 4)()
+    _lib.call("moe_fp8_matmul_plan", num_rows, out_cols, inner, _FORMAT[scale_format], info)
+    return dict(zip(("tokens_on_rows", "tile_cols", "splits", "ctas"), list(info)))
+
+
+def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
+               w2_scale: torch.Tensor, addend: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """The SwiGLU MLP of a shared expert on block-scaled e4m3 weights:
+    w2 (silu(w1 x) * (w3 x)) (+ addend), x [T, H] (f32/f16/bf16), w13 [2I, H]
+    (gate rows, then up rows), w2 [H, I]. Activations are quantised per token
+    and 128 columns in the weights' scale format; the gate-up product is held
+    in x's dtype. addend [T, H] in x's dtype (the routed experts' output) is
+    added before the one rounding of the result. Four launches."""
+    if w13.dim() != 2 or w2.dim() != 2 or w13.shape[0] != 2 * w2.shape[1]:
+        raise ValueError(f"w13 {tuple(w13.shape)} must be [2I, H] for w2 {tuple(w2.shape)}")
+    if w13_scale.dtype not in _SCALE_FORMAT:
+        raise ValueError("w13_scale must be float32 or uint8 (UE8M0)")
+    fmt = "fp32" if w13_scale.dtype == torch.float32 else "ue8m0"
+    both = block_matmul(*quantize_rows(x, fmt), w13, w13_scale, out_dtype=x.dtype)
+    return block_matmul(*quantize_rows(both, fmt, gated=True), w2, w2_scale, out_dtype=x.dtype,
+                        addend=addend, out=out)

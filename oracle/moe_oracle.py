@@ -436,3 +436,57 @@ def rel_l2(a: torch.Tensor, b: torch.Tensor) -> float:
     a = a.float().cpu()
     b = b.float().cpu()
     return float((a - b).norm() / b.norm().clamp_min(1e-30))
+
+
+# ---------------------------------------------------------------------------
+# Dense block-scaled fp8 (fp64 restatement)
+# ---------------------------------------------------------------------------
+
+def e4m3_nearest(v: torch.Tensor) -> torch.Tensor:
+    """v (fp64) to the nearest e4m3 value, halves to even, saturating at 448."""
+    e = torch.frexp(v.abs().clamp_min(2.0 ** -6)).exponent - 4
+    q = torch.ldexp(torch.round(torch.ldexp(v, -e)), e)
+    return torch.where(v.isnan(), v, q.clamp(-FP8_MAX, FP8_MAX))
+
+
+def _fp8_group(part: torch.Tensor, m: torch.Tensor, fmt: str):
+    """(q, scale), both fp64, of a group with absolute maximum m."""
+    s = torch.where(m > 0, m / FP8_MAX, torch.ones_like(m))
+    if fmt == "fp32":
+        return e4m3_nearest(part * FP8_MAX / torch.where(m > 0, m, torch.full_like(m, FP8_MAX))), s
+    frac, exp = torch.frexp(s)  # s = frac * 2^exp, 0.5 <= frac < 1
+    s = torch.ldexp(torch.ones_like(s), torch.where(frac == 0.5, exp - 1, exp))
+    return e4m3_nearest(part / s), s
+
+
+def fp8_rows(x: torch.Tensor, fmt: str):
+    """Per row and 128 columns: (q fp64 [T, K], scale fp64 [T, KB])."""
+    got = [_fp8_group(p, p.abs().amax(1, keepdim=True), fmt) for p in x.double().split(128, 1)]
+    return torch.cat([q for q, _ in got], 1), torch.cat([s for _, s in got], 1)
+
+
+def fp8_blocks(w: torch.Tensor, fmt: str):
+    """Per 128x128 block: (q fp64 [N, K], scale fp64 [NB, KB])."""
+    qs, ss = [], []
+    for band in w.double().split(128, 0):
+        got = [_fp8_group(p, p.abs().max().view(1, 1), fmt) for p in band.split(128, 1)]
+        qs.append(torch.cat([q for q, _ in got], 1))
+        ss.append(torch.cat([s for _, s in got], 1))
+    return torch.cat(qs), torch.cat(ss)
+
+
+def fp8_scale_values(scale: torch.Tensor) -> torch.Tensor:
+    """Stored scales (float32, or UE8M0 bytes) as fp64 numbers."""
+    if scale.dtype == torch.uint8:
+        return torch.ldexp(torch.ones(scale.shape, dtype=torch.float64), scale.int() - 127)
+    return scale.double()
+
+
+def fp8_dense(x, xs, w, ws):
+    """(product fp64 [T, N], sum of the terms' magnitudes [T, N]) of
+    block-scaled e4m3 operands with stored scales."""
+    (T, K), N = x.shape, w.shape[0]
+    a = x.double() * fp8_scale_values(xs).repeat_interleave(128, 1)[:, :K]
+    b = w.double() * (fp8_scale_values(ws).repeat_interleave(128, 0)[:N]
+                      .repeat_interleave(128, 1)[:, :K])
+    return a @ b.t(), a.abs() @ b.abs().t()

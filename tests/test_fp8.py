@@ -1,0 +1,86 @@
+"""CPU: refusals of the dense fp8 entry points (on the host, before any
+launch), the plan of the product, and the oracle's roundings."""
+import pytest
+import torch
+
+from kernelswift_b200 import _lib, fp8
+from oracle import moe_oracle as orc
+
+F32, BF16, I8 = _lib.DT_F32, _lib.DT_BF16, _lib.DT_I8
+INVALID, UNSUPPORTED = _lib.MOE_ERR_INVALID_ARG, _lib.MOE_ERR_UNSUPPORTED
+
+
+def quantize(x_dtype=BF16, T=4, K=256, ld=None, gated=0, fmt=1, q=0x1000, ld_q=256):
+    ld = (2 * K if gated else K) if ld is None else ld
+    return _lib.load().moe_fp8_quantize_rows(0x1000, x_dtype, T, K, ld, gated, fmt, q, ld_q,
+                                             0x1000, 4, 1, None)
+
+
+def matmul(x=0x1000, ld_x=256, w=0x1000, ld_w=256, fmt=1, T=4, N=64, K=256, add=None, ld_add=0,
+           ld_out=64, out_dtype=BF16):
+    return _lib.load().moe_fp8_matmul(x, ld_x, 0x1000, 4, 1, w, ld_w, 0x1000, fmt, T, N, K, add,
+                                      ld_add, 0x1000, ld_out, out_dtype, None, None)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(x_dtype=I8), INVALID), (dict(T=-1), INVALID), (dict(K=0), INVALID),
+    (dict(ld=255), INVALID), (dict(gated=1, ld=511), INVALID), (dict(fmt=2), INVALID),
+    (dict(q=0x1008), INVALID), (dict(ld_q=250), INVALID), (dict(K=257, ld_q=256), INVALID),
+    (dict(T=1 << 31), UNSUPPORTED),
+])
+def test_quantizer_refusals(bad, status):
+    assert quantize(**bad) == status
+    assert "fp8_quantize_rows" in _lib.load().moe_last_error().decode()
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(x=0x1008), INVALID), (dict(w=0x1004), INVALID), (dict(ld_x=250, K=250), INVALID),
+    (dict(ld_w=264), INVALID), (dict(ld_x=240), INVALID), (dict(fmt=3), INVALID),
+    (dict(T=-1), INVALID), (dict(N=0), INVALID), (dict(K=0), INVALID),
+    (dict(ld_out=63), INVALID), (dict(add=0x1000, ld_add=63), INVALID),
+    (dict(out_dtype=I8), INVALID), (dict(T=1 << 31), UNSUPPORTED), (dict(N=1 << 31), UNSUPPORTED),
+    (dict(T=1 << 30, N=1 << 30, ld_out=1 << 30), UNSUPPORTED),
+])
+def test_product_refusals(bad, status):
+    assert matmul(**bad) == status
+    assert "fp8_matmul" in _lib.load().moe_last_error().decode()
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError):
+        fp8.quantize_rows(torch.zeros(2, 128))
+    with pytest.raises(ValueError):
+        fp8.quantize_blocks(torch.zeros(2, 128))
+
+
+@pytest.mark.parametrize("fmt", ["fp32", "ue8m0"])
+def test_plan_covers_the_product(fmt):
+    """Every plan's tiles cover the output, K splits leave no CTA empty and
+    clusters stay within 8 CTAs."""
+    for T in (1, 2, 15, 16, 17, 64, 100, 128, 129, 300, 1000, 4096, 16384):
+        for N in (1, 100, 576, 4096, 7168, 100000):
+            for K in (1, 100, 1024, 2048, 7168, 20000):
+                p = fp8.block_matmul_plan(T, N, K, fmt)
+                kb = -(-K // 128)
+                assert 1 <= p["splits"] <= min(8, kb)
+                assert p["tile_cols"] in (16, 32, 64, 128, 256)
+                if p["tokens_on_rows"]:
+                    tiles = -(-T // 128) * -(-N // p["tile_cols"])
+                else:
+                    tiles = -(-T // p["tile_cols"]) * -(-N // 128)
+                if p["splits"] > 1:
+                    assert p["ctas"] == tiles * p["splits"]
+                else:
+                    assert 1 <= p["ctas"] <= min(tiles, 296)
+    assert fp8.block_matmul_plan(0, 64, 64, fmt)["ctas"] == 0
+
+
+def test_oracle_roundings():
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    every = every[~every.isnan()]
+    assert torch.equal(orc.e4m3_nearest(every), every)
+    v = torch.randn(10000, generator=torch.Generator().manual_seed(0)).double() * 100
+    assert torch.equal(orc.e4m3_nearest(v), v.clamp(-448, 448).to(torch.float8_e4m3fn).double())
+    q, s = orc.fp8_rows(torch.tensor([[448.0, 1.0], [449.0, 0.0], [0.0, 0.0]]), "ue8m0")
+    assert s.tolist() == [[1.0], [2.0], [1.0]]
+    assert q.tolist() == [[448.0, 1.0], [224.0, 0.0], [0.0, 0.0]]
