@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .fused_moe import _check_cuda, _code, _contig, _DTYPE_CODE, _ptr, _stream
+from .fused_moe import _check_cuda, _DTYPE_CODE, _enqueue
 
 _FORMAT = {"fp32": 0, "ue8m0": 1}
 _SCALE_FORMAT = {torch.float32: 0, torch.uint8: 1}
@@ -28,13 +28,19 @@ def _round_up(n: int, m: int) -> int:
     return -(-n // m) * m
 
 
+def _empty_fp8(rows: int, cols: int, device) -> torch.Tensor:
+    """[rows, cols] e4m3 whose rows start on 16-byte boundaries."""
+    q = torch.empty(rows, _round_up(cols, 16), dtype=torch.float8_e4m3fn, device=device)
+    return q if cols % 16 == 0 else q[:, :cols]
+
+
 def _no_grad_needed(name: str, t: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and t.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient; the fp8 operators have none "
                          "(call them under torch.no_grad())")
 
 
-def _rows_of(name: str, t: torch.Tensor) -> torch.Tensor:
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """A 2-D tensor whose rows are dense: `t`, or a dense copy."""
     if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.numel() == 0:
         return t
@@ -50,9 +56,9 @@ def _fp8_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= cols
             and t.data_ptr() % 16 == 0):
         return t
-    q = torch.empty(rows, _round_up(cols, 16), dtype=t.dtype, device=t.device)
-    q[:, :cols].view(torch.uint8).copy_(t.view(torch.uint8))
-    return q[:, :cols]
+    q = _empty_fp8(rows, cols, t.device)
+    q.view(torch.uint8).copy_(t.view(torch.uint8))
+    return q
 
 
 def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = False
@@ -69,22 +75,22 @@ def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = Fa
         raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
     if x.dim() != 2 or x.dtype not in _FLOAT or (gated and x.shape[1] % 2):
         raise ValueError("x must be a 2-D f32/f16/bf16 tensor, of an even width when gated")
-    x = _rows_of("x", x)
+    x = _rows_of(x)
     T = x.shape[0]
     K = x.shape[1] // 2 if gated else x.shape[1]
     if K < 1:
         raise ValueError("x has no columns")
     dev, kb = x.device, -(-K // 128)
-    q = torch.empty(T, _round_up(K, 16), dtype=torch.float8_e4m3fn, device=dev)
+    q = _empty_fp8(T, K, dev)
     if scale_format == "fp32":
-        scale = torch.empty(kb, _round_up(T, 4), dtype=torch.float32, device=dev).t()[:T]
+        strides, dtype = (1, _round_up(T, 4)), torch.float32
     else:
-        scale = torch.empty(T, _round_up(kb, 4), dtype=torch.uint8, device=dev)[:, :kb]
-    with torch.cuda.device(dev):
-        _lib.call("moe_fp8_quantize_rows", _ptr(x), _code(x), T, K, max(x.stride(0), x.shape[1]),
-                  int(gated), _FORMAT[scale_format], _ptr(q), q.stride(0), _ptr(scale),
-                  scale.stride(0), scale.stride(1), _stream(dev))
-    return q[:, :K], scale
+        strides, dtype = (_round_up(kb, 4), 1), torch.uint8
+    scale = torch.empty_strided((T, kb), strides, dtype=dtype, device=dev)
+    _enqueue("moe_fp8_quantize_rows", x.get_device(), x.data_ptr(), _DTYPE_CODE[x.dtype], T, K,
+             max(x.stride(0), x.shape[1]), gated, _FORMAT[scale_format], q.data_ptr(),
+             _round_up(K, 16), scale.data_ptr(), *strides)
+    return q, scale
 
 
 def quantize_blocks(w: torch.Tensor, scale_format: str = "ue8m0"
@@ -98,16 +104,16 @@ def quantize_blocks(w: torch.Tensor, scale_format: str = "ue8m0"
         raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
     if w.dim() != 2 or w.dtype not in _FLOAT or w.numel() == 0:
         raise ValueError("w must be a 2-D f32/f16/bf16 tensor")
-    w = _rows_of("w", w.detach())
+    w = _rows_of(w.detach())
     N, K = w.shape
     dev = w.device
-    q = torch.empty(N, _round_up(K, 16), dtype=torch.float8_e4m3fn, device=dev)
+    q = _empty_fp8(N, K, dev)
     scale = torch.empty(-(-N // 128), -(-K // 128), device=dev,
                         dtype=torch.float32 if scale_format == "fp32" else torch.uint8)
-    with torch.cuda.device(dev):
-        _lib.call("moe_fp8_quantize_blocks", _ptr(w), _code(w), N, K, max(w.stride(0), K),
-                  _FORMAT[scale_format], _ptr(q), q.stride(0), _ptr(scale), _stream(dev))
-    return q[:, :K], scale
+    _enqueue("moe_fp8_quantize_blocks", w.get_device(), w.data_ptr(), _DTYPE_CODE[w.dtype], N, K,
+             max(w.stride(0), K), _FORMAT[scale_format], q.data_ptr(), _round_up(K, 16),
+             scale.data_ptr())
+    return q, scale
 
 
 def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -124,42 +130,48 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     dtype and may be out itself. Summed in fp32, rounded once to out_dtype
     (bf16, f16 or f32). status: optional int32 device word (moe_read_status).
     """
+    index = x.get_device()
     for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
-        _check_cuda(name, t)
-        if t.device != x.device:
+        if t.get_device() != index or index < 0:
+            _check_cuda(name, t)
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
     x, w = _fp8_rows("x", x), _fp8_rows("w", w)
     (T, K), N = x.shape, w.shape[0]
-    kb = -(-K // 128)
+    kb, nb = -(-K // 128), -(-N // 128)
     if w.shape[1] != K or K < 1 or N < 1:
         raise ValueError(f"w {tuple(w.shape)} does not match x {tuple(x.shape)}")
-    if x_scale.dtype not in _SCALE_FORMAT or w_scale.dtype != x_scale.dtype:
+    fmt = _SCALE_FORMAT.get(x_scale.dtype)
+    if fmt is None or w_scale.dtype != x_scale.dtype:
         raise ValueError("x_scale and w_scale must both be float32 or both uint8 (UE8M0)")
-    if x_scale.shape != (T, kb) or w_scale.shape != (-(-N // 128), kb):
-        raise ValueError(f"scales must be [T, {kb}] and [{-(-N // 128)}, {kb}], got "
+    if x_scale.shape != (T, kb) or w_scale.shape != (nb, kb):
+        raise ValueError(f"scales must be [{T}, {kb}] and [{nb}, {kb}], got "
                          f"{tuple(x_scale.shape)} and {tuple(w_scale.shape)}")
-    if out is not None:
-        out_dtype = out.dtype
-    if out_dtype not in _FLOAT:
-        raise ValueError("out_dtype must be bf16, f16 or f32")
-    dev = x.device
     if out is None:
-        out = torch.empty(T, N, dtype=out_dtype, device=dev)
-    elif (out.shape != (T, N) or out.device != dev or out.stride(1) != 1
-          or out.stride(0) < N and T > 1):
-        raise ValueError(f"out must be a [{T}, {N}] tensor with dense rows on {dev}")
+        if out_dtype not in _FLOAT:
+            raise ValueError("out_dtype must be bf16, f16 or f32")
+        out = torch.empty(T, N, dtype=out_dtype, device=x.device)
+    else:
+        out_dtype = out.dtype
+        if (out.shape != (T, N) or out.get_device() != index or out_dtype not in _FLOAT
+                or out.stride(1) != 1 and N > 1 or out.stride(0) < N and T > 1):
+            raise ValueError(f"out must be a bf16, f16 or f32 [{T}, {N}] tensor with dense rows "
+                             f"on {x.device}")
+        _no_grad_needed("out", out)
+    add_ptr = add_ld = 0
     if addend is not None:
         _no_grad_needed("addend", addend)
-        if addend.shape != (T, N) or addend.dtype != out_dtype or addend.device != dev:
-            raise ValueError(f"addend must be a {out_dtype} [{T}, {N}] tensor on {dev}")
-        addend = _rows_of("addend", addend)
-    w_scale = w_scale if w_scale.is_contiguous() else w_scale.contiguous()
-    with torch.cuda.device(dev):
-        _lib.call("moe_fp8_matmul", _ptr(x), max(x.stride(0), _round_up(K, 16)), _ptr(x_scale),
-                  x_scale.stride(0), x_scale.stride(1), _ptr(w), max(w.stride(0), _round_up(K, 16)),
-                  _ptr(w_scale), _SCALE_FORMAT[x_scale.dtype], T, N, K, _ptr(addend),
-                  0 if addend is None else max(addend.stride(0), N), _ptr(out),
-                  max(out.stride(0), N), _DTYPE_CODE[out_dtype], _ptr(status), _stream(dev))
+        if addend.shape != (T, N) or addend.dtype != out_dtype or addend.get_device() != index:
+            raise ValueError(f"addend must be a {out_dtype} [{T}, {N}] tensor on {x.device}")
+        addend = _rows_of(addend)
+        add_ptr, add_ld = addend.data_ptr(), max(addend.stride(0), N)
+    if not w_scale.is_contiguous():
+        w_scale = w_scale.contiguous()
+    pitch = _round_up(K, 16)
+    _enqueue("moe_fp8_matmul", index, x.data_ptr(), max(x.stride(0), pitch), x_scale.data_ptr(),
+             x_scale.stride(0), x_scale.stride(1), w.data_ptr(), max(w.stride(0), pitch),
+             w_scale.data_ptr(), fmt, T, N, K, add_ptr or None, add_ld, out.data_ptr(),
+             max(out.stride(0), N), _DTYPE_CODE[out_dtype],
+             None if status is None else status.data_ptr())
     return out
 
 

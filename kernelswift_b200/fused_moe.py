@@ -57,6 +57,16 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def _enqueue(entry: str, index: int, *args) -> None:
+    """Calls a library entry point on the current stream of device `index`,
+    that device made current for the call."""
+    if torch.cuda.current_device() == index:
+        _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def _check_cuda(name: str, t: torch.Tensor) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
@@ -158,20 +168,26 @@ _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
 
 
+def _launch_balanced(logits, bias, topk, renormalize, groups, kept, scoring, group_score, scale,
+                     load, weights_dtype, ids_dtype):
+    T, E = logits.shape
+    w = torch.empty(T, topk, dtype=weights_dtype, device=logits.device)
+    ids = torch.empty(T, topk, dtype=ids_dtype, device=logits.device)
+    _enqueue("moe_balanced_topk", logits.get_device(), logits.data_ptr(), _code(logits),
+             None if bias is None else bias.data_ptr(), T, E, topk, renormalize, groups, kept,
+             group_score, scoring, scale, w.data_ptr(), _code(w), ids.data_ptr(), _code(ids),
+             None if load is None else load.data_ptr())
+    return w, ids
+
+
 class _BalancedTopK(torch.autograd.Function):
     """moe_balanced_topk with moe_balanced_topk_backward as its gradient."""
 
     @staticmethod
     def forward(ctx, logits, bias, topk, renormalize, groups, kept, scoring, group_score, scale,
                 load, weights_dtype, ids_dtype):
-        T, E = logits.shape
-        dev = logits.device
-        w = torch.empty(T, topk, dtype=weights_dtype, device=dev)
-        ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("moe_balanced_topk", _ptr(logits), _code(logits), _ptr(bias), T, E, topk,
-                      renormalize, groups, kept, group_score, scoring, scale, _ptr(w), _code(w),
-                      _ptr(ids), _code(ids), _ptr(load), _stream(dev))
+        w, ids = _launch_balanced(logits, bias, topk, renormalize, groups, kept, scoring,
+                                  group_score, scale, load, weights_dtype, ids_dtype)
         ctx.args = (topk, renormalize, scoring, scale)
         ctx.save_for_backward(logits, ids)
         ctx.mark_non_differentiable(ids)
@@ -181,14 +197,13 @@ class _BalancedTopK(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_w, _grad_ids):
         logits, ids = ctx.saved_tensors
-        topk, renormalize, scoring, scale = ctx.args
         T, E = logits.shape
         grad_w = grad_w.to(torch.float32).contiguous()
         grad = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
-        with torch.cuda.device(logits.device):
-            _lib.call("moe_balanced_topk_backward", _ptr(logits), _code(logits), _ptr(ids),
-                      _code(ids), _ptr(grad_w), T, E, topk, renormalize, scoring, scale,
-                      _ptr(grad), _stream(logits.device))
+        topk, renormalize, scoring, scale = ctx.args
+        _enqueue("moe_balanced_topk_backward", logits.get_device(), logits.data_ptr(),
+                 _code(logits), ids.data_ptr(), _code(ids), grad_w.data_ptr(), T, E, topk,
+                 renormalize, scoring, scale, grad.data_ptr())
         return (grad,) + (None,) * 11
 
 
@@ -224,18 +239,22 @@ def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
         raise ValueError(f"Unsupported scoring_func: {scoring_func}")
     if group_score not in _GROUP_SCORE:
         raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORE)}")
-    E, dev = gating_output.shape[1], gating_output.device
+    E = gating_output.shape[1]
     for name, t, dtype in (("expert_bias", expert_bias, torch.float32),
                            ("expert_load", expert_load, torch.int32)):
-        if t is not None and (t.dtype != dtype or t.shape != (E,) or t.device != dev):
-            raise ValueError(f"{name} must be a {dtype} [E] = [{E}] tensor on {dev}")
+        if t is not None and (t.dtype != dtype or t.shape != (E,)
+                              or t.get_device() != gating_output.get_device()):
+            raise ValueError(f"{name} must be a {dtype} [E] = [{E}] tensor on "
+                             f"{gating_output.device}")
     if expert_load is not None and not expert_load.is_contiguous():
         raise ValueError("expert_load must be contiguous (it is added to in place)")
     bias = None if expert_bias is None else _contig(expert_bias.detach())
-    return _BalancedTopK.apply(_contig(gating_output), bias, topk, int(renormalize),
-                               num_expert_group, topk_group, _SCORING[scoring_func],
-                               _GROUP_SCORE[group_score], float(routed_scaling_factor),
-                               expert_load, weights_dtype, ids_dtype)
+    run = _launch_balanced
+    if gating_output.requires_grad and torch.is_grad_enabled():
+        run = _BalancedTopK.apply
+    return run(_contig(gating_output), bias, topk, int(renormalize), num_expert_group, topk_group,
+               _SCORING[scoring_func], _GROUP_SCORE[group_score], float(routed_scaling_factor),
+               expert_load, weights_dtype, ids_dtype)
 
 
 # ---------------------------------------------------------------------------
