@@ -37,6 +37,8 @@ constexpr int kABytes = kLanes * kKB;
 constexpr int kSfSlots = 4;         // scale ring: quads of 4 k-blocks (UE8M0)
 constexpr int kFacSlots = 8;        // scale ring: k-blocks (fp32)
 
+constexpr int kStagedBytes = 4096;  // staged tokens of one epilogue group (two such buffers)
+
 struct MatmulParams {
   const void* xs;  // activation scales, f32 or bytes
   int64_t xs_row, xs_blk;
@@ -138,7 +140,8 @@ struct ColsCfg {
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kSfb = (BN + 127) / 128;       // scale chunks of the tokens
   static constexpr int kRingBytes = MX ? kSfSlots * 512 * (1 + kSfb) : kFacSlots * BN * 4;
-  static constexpr size_t kFixed = 1024 + 512 + kRingBytes;
+  static constexpr int kGroups = kEpiWarps / 4;       // epilogue groups of 128 lanes
+  static constexpr size_t kFixed = 1024 + 512 + kRingBytes + size_t(kGroups) * 2 * kStagedBytes;
   static constexpr int kStages = int(((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / kStageBytes);
   static constexpr size_t kSmem = kFixed + size_t(kStages) * kStageBytes;
   // TMEM: accumulators (UE8M0) or per-k-block buffers (fp32), then scale slots
@@ -169,7 +172,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   uint8_t* sA = smem;
   uint8_t* sB = sA + STAGES * kABytes;
   uint8_t* sRing = sB + STAGES * C::kBBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sRing + C::kRingBytes);
+  uint8_t* sOut = sRing + C::kRingBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + C::kGroups * 2 * kStagedBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* sfull = empty + STAGES;
   uint64_t* sempty = sfull + SLOTS;
@@ -222,21 +226,68 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
   bool epi_ok = true;
 
-  auto store_tile = [&](const Tile& tile, int col0, int row) {
-    const int64_t n = int64_t(tile.n) * kLanes + row;
+  // 16-byte stores when every output row starts on such a boundary
+  constexpr int kVec = 16 / int(sizeof(TOUT));
+  const bool vec = p.ld_out % kVec == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+
+  // Writes the tile's columns (tokens) col0 .. col0 + COLS of this epilogue
+  // group's 128 lanes (weight rows, neighbours in the output). A lane holds
+  // one output column of every token; tokens go through shared memory, a few
+  // at a time, so that a warp stores whole 128-byte lines.
+  auto store_tile = [&](const Tile& tile, int col0, int row, int group) {
+    const int64_t n0 = int64_t(tile.n) * kLanes;
     const int64_t t0 = int64_t(tile.t) * BN + col0;
-    if (n >= p.N) return;
-    TOUT* out = static_cast<TOUT*>(p.out) + t0 * p.ld_out + n;
-    const TOUT* add = static_cast<const TOUT*>(p.add) + t0 * p.ld_add + n;
-    const int live = int(min(int64_t(COLS), p.T - t0));
+    const int64_t live = min(int64_t(COLS), p.T - t0);
+    const bool in = n0 + row < p.N;
+    TOUT* out = static_cast<TOUT*>(p.out) + t0 * p.ld_out + n0;
+    if (p.add != nullptr) {
+      const TOUT* add = static_cast<const TOUT*>(p.add) + t0 * p.ld_add + n0 + row;
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) {
-      if (j < live) {
-        float v = acc[j];
-        if (p.add != nullptr) v += to_f32(add[j * p.ld_add]);
-        out[j * p.ld_out] = from_f32<TOUT>(v);
+      for (int j = 0; j < COLS; ++j) {
+        if (in && j < live) acc[j] += to_f32(*add);
+        add += p.ld_add;
       }
     }
+    if (!vec) {
+      out += row;
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) {
+        if (in && j < live) *out = from_f32<TOUT>(acc[j]);
+        out += p.ld_out;
+      }
+      return;
+    }
+    constexpr int TOK = kStagedBytes / (kLanes * int(sizeof(TOUT)));  // tokens per buffer
+    constexpr int SEGS = kLanes / kVec;                               // vectors per token
+    TOUT* staged = reinterpret_cast<TOUT*>(sOut + group * 2 * kStagedBytes);
+#pragma unroll
+    for (int c = 0; c < COLS; c += TOK) {
+      if (c >= live) break;
+      TOUT* buf = staged + ((c / TOK) & 1) * (TOK * kLanes);
+#pragma unroll
+      for (int j = 0; j < TOK; ++j) buf[j * kLanes + row] = from_f32<TOUT>(acc[c + j]);
+      // the buffer's readers of two chunks ago passed the last chunk's barrier
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+#pragma unroll
+      for (int i = 0; i < TOK * SEGS / 128; ++i) {
+        const int v = row + 128 * i;
+        const int j = v / SEGS, seg = v % SEGS;
+        const uint4 w = reinterpret_cast<const uint4*>(buf)[v];
+        if (c + j >= live) continue;
+        TOUT* dst = out + (c + j) * p.ld_out + seg * kVec;
+        const int64_t left = p.N - n0 - seg * kVec;
+        if (left >= kVec) {
+          *reinterpret_cast<uint4*>(dst) = w;
+        } else {
+          const TOUT* e = reinterpret_cast<const TOUT*>(&w);
+#pragma unroll
+          for (int k = 0; k < kVec; ++k)
+            if (k < left) dst[k] = e[k];
+        }
+      }
+    }
+    // the next tile starts with buffer 0 again
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
   };
 
   if (warp == 0 && lane == 0) {
@@ -499,7 +550,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
         if (!epi_ok) break;
       }
       if (p.splits == 1) {
-        store_tile(tile, col0, row);
+        store_tile(tile, col0, row, (warp - 4) >> 2);
       } else {
         // every MMA of this CTA's only tile has completed, so the stages are
         // free; [token][weight row], a warp writes 32 neighbouring words
