@@ -521,7 +521,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
               tmem_ld32(base + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
             else
               tmem_ld16(base + c, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
-            tmem_arrived(v);
+            // the factors are read after it, so no product can move before it
+            tmem_ld_wait();
             if (c + BATCH >= COLS) {
               tc_fence_before();
               __syncwarp();
@@ -611,7 +612,46 @@ struct RowsCfg {
   static constexpr int kStages = 4;
   static constexpr size_t kSmem = 1024 + 256 + size_t(kStages) * kStageBytes;
   static constexpr int kBufs = 2;
+  // The block launches at kLaunchRegs registers per thread; the control
+  // warpgroup gives registers back and the 16 epilogue warps take them, for 64
+  // sums and a batch of 32 partials each. The split adds up to the launch's
+  // total, which the host checks against the compiled kernel.
+  static constexpr int kLaunchRegs = 96, kCtrlRegs = 32, kEpiRegs = 112;
+  static_assert(128 * kCtrlRegs + 32 * kEpiWarps * kEpiRegs == kThreads * kLaunchRegs,
+                "setmaxnreg split");
 };
+
+// Transposes 4 x 4 vectors among the lanes of a quad: lane i's vector c
+// becomes lane c's vector i (its own inverse).
+__device__ __forceinline__ uint4 shfl_xor4(const uint4& v, int m) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m),
+                    __shfl_xor_sync(0xffffffffu, v.z, m), __shfl_xor_sync(0xffffffffu, v.w, m));
+}
+__device__ __forceinline__ uint4 pick(bool b, const uint4& x, const uint4& y) {
+  return make_uint4(b ? x.x : y.x, b ? x.y : y.y, b ? x.z : y.z, b ? x.w : y.w);
+}
+__device__ __forceinline__ void swap_pair(uint4& lo, uint4& hi, bool up, int m) {
+  const uint4 got = shfl_xor4(pick(up, lo, hi), m);
+  lo = pick(up, got, lo);
+  hi = pick(up, hi, got);
+}
+__device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
+  swap_pair(v[0], v[1], lane & 1, 1);
+  swap_pair(v[2], v[3], lane & 1, 1);
+  swap_pair(v[0], v[2], lane & 2, 2);
+  swap_pair(v[1], v[3], lane & 2, 2);
+}
+
+// 16 bytes of the output's type to and from fp32.
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* x) {
+  if constexpr (std::is_same<T, float>::value)
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                      __float_as_uint(x[3]));
+  else
+    return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                      pack2<T>(x[6], x[7]));
+}
 
 template <typename TOUT>
 __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
@@ -621,7 +661,7 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
   constexpr int STAGES = C::kStages;
   constexpr int NB = C::kBufs;
   constexpr int COLS = C::kCols;
-  constexpr int BATCH = 16;
+  constexpr int BATCH = 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -664,6 +704,7 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
   const int tiles = p.t_tiles * p.n_tiles;
   const int kbs = p.kb_total;
 
+  if (warp < 4) setmaxnreg_dec<C::kCtrlRegs>();
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmX);
     tma_prefetch_desc(&tmW);
@@ -724,6 +765,7 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
     volatile int no_abort = 0;
     mbar_wait_bounded(final_bar, 0, &no_abort, limit);
   } else if (warp >= 4) {
+    setmaxnreg_inc<C::kEpiRegs>();
     const int row = (warp & 3) * 32 + lane;
     const int col0 = ((warp - 4) >> 2) * COLS;
     const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(col0);
@@ -733,6 +775,7 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
     // 16-byte stores when every output row starts on such a boundary
     constexpr int kVec = 16 / int(sizeof(TOUT));
     const bool vec = p.ld_out % kVec == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+    const bool add_vec = p.ld_add % kVec == 0 && (reinterpret_cast<uintptr_t>(p.add) & 15) == 0;
     int buf = 0;
     uint32_t bphase = 0;
     bool ok = true;
@@ -750,7 +793,7 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
       // the next k-block's scales are on their way while this one is added
       float sx_n = __ldg(sx), sw_n = __ldg(sw);
       for (int kb = 0; kb < kbs; ++kb) {
-        const float s = sx_n * sw_n;
+        float s = sx_n * sw_n;
         if (kb + 1 < kbs) {
           sx_n = __ldg(sx + (kb + 1) * p.xs_blk);
           sw_n = __ldg(sw + kb + 1);
@@ -763,8 +806,9 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < COLS; c += BATCH) {
           uint32_t v[BATCH];
-          tmem_ld16(base + c, v);
-          tmem_arrived(v);
+          tmem_ld32(base + c, v);
+          tmem_ld_wait();
+          asm volatile("" : "+f"(s));  // no product can move before the wait
           if (c + BATCH >= COLS) {
             tc_fence_before();
             __syncwarp();
@@ -779,33 +823,53 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
           bphase ^= 1u;
         }
       }
-      if (!ok || !live) continue;
-      TOUT* out = static_cast<TOUT*>(p.out) + t * p.ld_out + n0;
-      const TOUT* add = static_cast<const TOUT*>(p.add) + t * p.ld_add + n0;
+      if (!ok) continue;
+      TOUT* out = static_cast<TOUT*>(p.out) + n0;
+      const TOUT* add = static_cast<const TOUT*>(p.add) + n0;
       const int cols = int(min(int64_t(COLS), max(int64_t(0), p.N - n0)));
-      if (p.add != nullptr) {
+      if (vec && cols == COLS && (p.add == nullptr || add_vec)) {
+        // a quad of lanes trades vectors so that it stores 64 bytes of one
+        // row at a time (and reads the addend so)
+        const int64_t t4 = t - (lane & 3);
+        const int mine = (lane & 3) * kVec;
 #pragma unroll
-        for (int j = 0; j < COLS; ++j)
-          if (j < cols) acc[j] += to_f32(add[j]);
-      }
-      if (vec && cols == COLS) {
+        for (int j = 0; j < COLS; j += 4 * kVec) {
+          uint4 v[4];
+          if (p.add != nullptr) {
 #pragma unroll
-        for (int j = 0; j < COLS; j += kVec) {
-          if constexpr (std::is_same<TOUT, float>::value)
-            *reinterpret_cast<float4*>(out + j) =
-                make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-          else
-            *reinterpret_cast<uint4*>(out + j) = make_uint4(
-                pack2<TOUT>(acc[j], acc[j + 1]), pack2<TOUT>(acc[j + 2], acc[j + 3]),
-                pack2<TOUT>(acc[j + 4], acc[j + 5]), pack2<TOUT>(acc[j + 6], acc[j + 7]));
+            for (int r = 0; r < 4; ++r)
+              v[r] = t4 + r < p.T ? *reinterpret_cast<const uint4*>(add + (t4 + r) * p.ld_add +
+                                                                    j + mine)
+                                  : make_uint4(0, 0, 0, 0);
+            quad_transpose(v, lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const TOUT* e = reinterpret_cast<const TOUT*>(&v[r]);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) acc[j + r * kVec + k] += to_f32(e[k]);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = pack16<TOUT>(&acc[j + r * kVec]);
+          quad_transpose(v, lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t4 + r < p.T)
+              *reinterpret_cast<uint4*>(out + (t4 + r) * p.ld_out + j + mine) = v[r];
         }
-      } else {
+      } else if (live) {
+        out += t * p.ld_out;
+        add += t * p.ld_add;
 #pragma unroll
         for (int j = 0; j < COLS; ++j)
-          if (j < cols) out[j] = from_f32<TOUT>(acc[j]);
+          if (j < cols) {
+            if (p.add != nullptr) acc[j] += to_f32(add[j]);
+            out[j] = from_f32<TOUT>(acc[j]);
+          }
       }
     }
   }
+  __syncwarp();
   __syncthreads();
   if (warp == 1) {
     __syncwarp();
@@ -925,6 +989,14 @@ int run_matmul(const Plan& plan, bool mx, const CUtensorMap& w, const CUtensorMa
     static std::atomic<uint64_t> done{0};
     int st = set_smem_once(fp8_rows_kernel<TOUT>, RowsCfg::kSmem, done);
     if (st != MOE_OK) return st;
+    // a register split that the launch cannot cover would never return
+    static const int regs = [] {
+      cudaFuncAttributes attr;
+      return cudaFuncGetAttributes(&attr, fp8_rows_kernel<TOUT>) == cudaSuccess ? attr.numRegs
+                                                                                : -1;
+    }();
+    KSW_REQUIRE(regs == RowsCfg::kLaunchRegs, MOE_ERR_UNSUPPORTED,
+                "fp8_matmul: compiled register count does not match the setmaxnreg split");
     return launch_clusters(fp8_rows_kernel<TOUT>, plan.ctas, RowsCfg::kThreads, RowsCfg::kSmem, 1,
                            s, x, w, p);
   }
