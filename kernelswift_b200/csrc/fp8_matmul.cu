@@ -3,25 +3,23 @@
 //                              sum_{k in block kb} xq[t, k] wq[n, k]
 // with e4m3 operands xq [T, K] and wq [N, K] on the tcgen05 tensor cores.
 //
-// Two kernels, by where the scales are applied and which operand lies on the
-// MMA's 128 rows (TMEM lanes):
+// UE8M0 scales are applied by the tensor core (kind::mxf8f6f4, block_scale):
+// all k-blocks of a tile accumulate in one TMEM accumulator. fp32 scales
+// cannot be: each k-block's product goes to a TMEM buffer of its own and is
+// added to fp32 registers times sx * sw. Two kernels:
 //
-// fp8_cols_kernel: a tile is 128 weight rows (lanes) x BN tokens (columns),
-//   BN in {16, ..., 256}, so that a handful of tokens costs a handful of
-//   columns. UE8M0 scales are applied by the tensor core (kind::mxf8f6f4,
-//   block_scale): all k-blocks accumulate in one TMEM accumulator. fp32 scales
-//   cannot be: each k-block's product goes to a TMEM buffer of its own and is
-//   added to fp32 registers times sx * sw, which a warp brings to shared
-//   memory per k-block (a column's factor is the same for all lanes). Tiles
-//   too few for the SMs are split along K over a cluster of up to 8 CTAs,
-//   whose fp32 partials are summed in rank order through distributed shared
-//   memory: one launch, no workspace, a fixed order of summation.
+// fp8_cols_kernel: a tile is 128 weight rows (TMEM lanes) x BN tokens
+//   (columns), BN in {16, ..., 256}, so that a handful of tokens costs a
+//   handful of columns. For fp32 scales a warp brings sx * sw of every column
+//   to shared memory per k-block (a column's factor is the same for all
+//   lanes). Tiles too few for the SMs are split along K over a cluster of up
+//   to 8 CTAs, whose fp32 partials are summed in rank order through
+//   distributed shared memory: one launch, no workspace, a fixed order.
 //
-// fp8_rows_kernel: fp32 scales and many tokens. A tile is 128 tokens (lanes) x
-//   256 weight rows (columns): a thread's columns share one sw and its row one
-//   sx, so the promotion needs a single factor per thread and k-block instead
-//   of one per column (shared-memory reads that would compete with the MMA's
-//   operand reads).
+// fp8_pair_kernel: many tokens. Two CTAs share a tile of 256 tokens (lanes) x
+//   256 weight rows (columns), each holding half of either operand; with fp32
+//   scales a thread's columns share one sw and its row one sx, a single factor
+//   per thread and k-block.
 #include <atomic>
 #include <type_traits>
 
@@ -34,8 +32,7 @@ namespace {
 constexpr int kKB = 128;            // bytes (= columns) of a k-block
 constexpr int kLanes = 128;         // rows of the MMA
 constexpr int kABytes = kLanes * kKB;
-constexpr int kSfSlots = 4;         // scale ring: quads of 4 k-blocks (UE8M0)
-constexpr int kFacSlots = 8;        // scale ring: k-blocks (fp32)
+constexpr int kFacSlots = 8;        // fp32 scale ring: k-blocks
 
 constexpr int kStagedBytes = 4096;  // staged tokens of one epilogue group (two such buffers)
 
@@ -95,6 +92,28 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
+// One lane of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
+// Barrier `id` of 128 threads; whether all of them came with `ok`. A warp that
+// gave up waiting takes part with false, so none is left at the barrier alone.
+__device__ __forceinline__ bool group_ok(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
+      "bar.red.and.pred p, %1, 128, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(uint32_t(ok))
+      : "memory");
+  return r != 0;
+}
+
 // Waits for this thread's tensor-memory loads; the values read pass through
 // the (empty) statements after it, so no use of them can move before it.
 template <int N>
@@ -104,28 +123,91 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 
-// The last phase of each stage of a TMA ring that issued `issued` boxes: waits
-// until none is in flight (a kernel must not end before its copies).
-__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, uint32_t issued,
-                                           uint64_t limit) {
-  for (int s = 0; s < stages; ++s) {
-    const uint32_t n = issued / stages + (uint32_t(s) < issued % stages ? 1u : 0u);
-    if (n == 0) continue;
-    volatile int no_abort = 0;
-    mbar_wait_bounded(&full[s], (n - 1) & 1u, &no_abort, limit);
+// The stages that the producers have filled, and the parity of each one's last
+// fill (whichever warp's), so that they can wait for the copies before they end.
+struct Filled {
+  uint32_t used = 0, parity = 0;
+  __device__ __forceinline__ void add(int stage, uint32_t phase) {
+    used |= 1u << stage;
+    parity = (parity & ~(1u << stage)) | (phase << stage);
   }
-}
+  __device__ __forceinline__ void drain(uint64_t* full, int stages, uint64_t limit) const {
+    for (int s = 0; s < stages; ++s)
+      if ((used >> s) & 1u) {
+        volatile int no_abort = 0;
+        mbar_wait_bounded(&full[s], (parity >> s) & 1u, &no_abort, limit);
+      }
+  }
+};
 
-// Four consecutive scale bytes 4q .. 4q + 3 of one row (bytes past KB are 0).
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int64_t stride, int q, int kb,
-                                               bool words) {
-  if (words && 4 * q + 4 <= kb) return __ldg(reinterpret_cast<const uint32_t*>(row + 4 * q));
-  uint32_t w = 0;
+// TMA producers: two warps take the stages in turn. A turn (wait for the
+// stage, announce its bytes, issue two copies) takes a warp about 490 cycles
+// whatever the boxes' size (570 from a single diverged lane), and a stage's
+// MMAs no more than 512, so one warp alone would starve the tensor core.
+constexpr int kProducers = 2;
+__device__ __forceinline__ int producer_of(int warp) { return warp == 0 ? 0 : warp == 3 ? 1 : -1; }
+
+// UE8M0 scales travel as words of four bytes, the scales of one row in a quad
+// of k-blocks. A loader warp builds the tensor core's 512-byte chunks (128
+// rows: lane l holds rows l, l + 32, l + 64, l + 96) of Q quads at a time:
+// some 16 loads under way per lane instead of four, since a turn of the loader
+// takes 2,000 to 3,600 cycles and a quad's MMAs only 2,048.
+template <int Q>
+struct ScaleWords {
+  uint32_t v[4][Q];
+
+  // The words of quads q0 .. q0 + Q of 128 rows of `scale` from row `row0`, of
+  // which those below `rows` exist; bytes past the KB blocks are 0.
+  __device__ __forceinline__ void fetch(const uint8_t* scale, int64_t row_stride,
+                                        int64_t blk_stride, bool words, int64_t row0,
+                                        int64_t rows, int lane, int q0, int kb) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (4 * q + i < kb) w |= uint32_t(__ldg(row + int64_t(4 * q + i) * stride)) << (8 * i);
-  return w;
-}
+    for (int r = 0; r < 4; ++r) {
+      const int64_t t = row0 + 32 * r + lane;
+      const uint8_t* at = scale + t * row_stride;
+#pragma unroll
+      for (int j = 0; j < Q; ++j) {
+        const int b = 4 * (q0 + j);
+        v[r][j] = 0;
+        if (t < rows) {
+          if (words && b + 4 <= kb) {
+            v[r][j] = __ldg(reinterpret_cast<const uint32_t*>(at + b));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (b + i < kb) v[r][j] |= uint32_t(__ldg(at + (b + i) * blk_stride)) << (8 * i);
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* chunk, int stride, int lane) const {
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+      reinterpret_cast<uint4*>(chunk + j * stride)[lane] =
+          make_uint4(v[0][j], v[1][j], v[2][j], v[3][j]);
+  }
+};
+
+// The same of one 128-row block of the weights, whose rows share their scale:
+// lane i < 4 Q holds byte i.
+template <int Q>
+struct BlockWords {
+  uint32_t byte;
+  __device__ __forceinline__ void fetch(const uint8_t* block, bool in, int lane, int q0, int kb) {
+    const int b = 4 * q0 + lane;
+    byte = in && lane < 4 * Q && b < kb ? __ldg(block + b) : 0u;
+  }
+  __device__ __forceinline__ void store(uint8_t* chunk, int stride, int lane) const {
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= __shfl_sync(0xffffffffu, byte, 4 * j + i) << (8 * i);
+      reinterpret_cast<uint4*>(chunk + j * stride)[lane] = make_uint4(w, w, w, w);
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------
 // fp8_cols_kernel
@@ -139,7 +221,12 @@ struct ColsCfg {
   static constexpr int kBBytes = BN * kKB;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kSfb = (BN + 127) / 128;       // scale chunks of the tokens
-  static constexpr int kRingBytes = MX ? kSfSlots * 512 * (1 + kSfb) : kFacSlots * BN * 4;
+  // UE8M0 scale ring: slots, and quads of k-blocks in each. A short run of
+  // k-blocks (a split tile's) starts sooner on small slots.
+  static constexpr int kSfSlots = 4, kQuads = 1;
+  static constexpr int kQuadBytes = 512 * (1 + kSfb);
+  static constexpr int kRingBytes =
+      MX ? kSfSlots * kQuads * kQuadBytes : kFacSlots * BN * 4;
   static constexpr int kGroups = kEpiWarps / 4;       // epilogue groups of 128 lanes
   static constexpr size_t kFixed = 1024 + 512 + kRingBytes + size_t(kGroups) * 2 * kStagedBytes;
   static constexpr int kStages = int(((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / kStageBytes);
@@ -148,7 +235,7 @@ struct ColsCfg {
   static constexpr int kBufs = MX ? (BN == 256 ? 1 : 2) : (BN == 256 ? 2 : 4);
   static constexpr int kSfCol0 = kBufs * BN;
   static constexpr int kSfCols = 4 * (1 + kSfb);
-  static constexpr int kUsed = kSfCol0 + (MX ? kSfSlots * kSfCols : 0);
+  static constexpr int kUsed = kSfCol0 + (MX ? kSfSlots * kQuads * kSfCols : 0);
   static constexpr int kTmem = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static_assert(kUsed <= 512 && kTmem * kCtas <= 512, "TMEM columns");
   static_assert(size_t(kStages) * kStageBytes >= size_t(BN) * kLanes * 4,
@@ -164,7 +251,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   constexpr int STAGES = C::kStages;
   constexpr int NB = C::kBufs;
   constexpr int COLS = C::kCols;
-  constexpr int SLOTS = MX ? kSfSlots : kFacSlots;
+  constexpr int SLOTS = MX ? C::kSfSlots : kFacSlots;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -183,7 +270,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5;
+  // the warp's number, known to be the same for all its lanes
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -191,7 +279,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&sfull[s], 32);
+      mbar_init(&sfull[s], 1);
       mbar_init(&sempty[s], MX ? 1 : C::kEpiWarps);
     }
     for (int b = 0; b < NB; ++b) {
@@ -286,85 +374,103 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
         }
       }
     }
-    // the next tile starts with buffer 0 again
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+    // the next tile starts with buffer 0 again, after its own group_ok
   };
 
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer ----------------
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
-    int stage = 0;
-    uint32_t phase = 0, issued = 0;
+  if (producer_of(warp) >= 0) {
+    // ---------------- TMA producers ----------------
+    const bool leader = elect_one();
+    if (leader) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+    }
+    const int mine = producer_of(warp);
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    Filled filled;
     bool ok = true;
     for (int i = first; ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, limit)) {
-          ok = false;
-          break;
+        if (turn == mine) {
+          ok = all_ok(mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, limit));
+          if (!ok) break;
+          if (leader) {
+            mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+            tma_load_2d(sA + stage * kABytes, &tmW, kb * kKB, tile.n * kLanes, &full[stage]);
+            tma_load_2d(sB + stage * C::kBBytes, &tmX, kb * kKB, tile.t * BN, &full[stage]);
+          }
+          __syncwarp();
         }
-        mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
-        tma_load_2d(sA + stage * kABytes, &tmW, kb * kKB, tile.n * kLanes, &full[stage]);
-        tma_load_2d(sB + stage * C::kBBytes, &tmX, kb * kKB, tile.t * BN, &full[stage]);
-        ++issued;
+        filled.add(stage, phase);
+        turn = turn + 1 == kProducers ? 0 : turn + 1;
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    drain_ring(full, STAGES, issued, limit);
-  } else if (warp == 1 && lane == 0) {
+    filled.drain(full, STAGES, limit);
+  } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
+    // The whole warp walks the loop and one lane issues: operands computed by
+    // a converged warp stay in uniform registers, where the MMA takes them.
+    const bool leader = elect_one();
+    const uint64_t desc_a = make_sw128_desc(smem_u32(sA));
+    const uint64_t desc_b = make_sw128_desc(smem_u32(sB));
     int stage = 0, buf = 0, slot = 0;
+    [[maybe_unused]] uint32_t sf = 0;  // TMEM of the quad's scales
     uint32_t phase = 0, bphase = 0, sphase = 0;
     bool ok = true;
     for (int i = first; ok && i < tiles; i += step) {
       if constexpr (MX) {
-        if (!mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit)) break;
+        if (!all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit))) break;
         tc_fence_after();
       }
       for (int kb = kb0; kb < kb1; ++kb) {
         if constexpr (MX) {
-          if (kb == kb0 || (kb & 3) == 0) {
-            if (!mbar_wait_bounded(&sfull[slot], sphase, abort_flag, limit)) {
-              ok = false;
-              break;
-            }
+          if (kb == kb0 || kb % (4 * C::kQuads) == 0) {
+            ok = all_ok(mbar_wait_bounded(&sfull[slot], sphase, abort_flag, limit));
+            if (!ok) break;
             tc_fence_after();
+          }
+          if (kb == kb0 || (kb & 3) == 0) {
             // a slot's TMEM columns are rewritten only after sempty, i.e. after
             // the MMAs that read them completed
-            const uint32_t sf = tmem_base + uint32_t(C::kSfCol0 + slot * C::kSfCols);
-            const uint32_t src = smem_u32(sRing + slot * 512 * (1 + C::kSfb));
+            const int quad = slot * C::kQuads + (kb >> 2) % C::kQuads;
+            sf = tmem_base + uint32_t(C::kSfCol0 + quad * C::kSfCols);
+            const uint32_t src = smem_u32(sRing + quad * C::kQuadBytes);
+            if (leader) {
 #pragma unroll
-            for (int c = 0; c < 1 + C::kSfb; ++c)
-              tc_cp_sf(sf + 4 * c, make_sf_desc(src + 512 * c));
+              for (int c = 0; c < 1 + C::kSfb; ++c)
+                tc_cp_sf(sf + 4 * c, make_sf_desc(src + 512 * c));
+            }
+            __syncwarp();
           }
         } else {
-          if (!mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit)) {
-            ok = false;
-            break;
-          }
+          ok = all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit));
+          if (!ok) break;
         }
-        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, limit)) {
-          ok = false;
-          break;
-        }
+        ok = all_ok(mbar_wait_bounded(&full[stage], phase, abort_flag, limit));
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem_base + uint32_t(buf * BN);
-        const uint32_t a0 = smem_u32(sA + stage * kABytes);
-        const uint32_t b0 = smem_u32(sB + stage * C::kBBytes);
+        // descriptors of the stage's tiles; 32 bytes further along K are 2 units
+        const uint64_t a0 = desc_a + uint32_t(stage * (kABytes / 16));
+        const uint64_t b0 = desc_b + uint32_t(stage * (C::kBBytes / 16));
         if constexpr (MX) {
-          const uint32_t sf = tmem_base + uint32_t(C::kSfCol0 + slot * C::kSfCols);
           const uint32_t idesc = idesc_sf_ids(make_idesc_mx(kLanes, BN), uint32_t(kb & 3));
+          const bool slot_end = kb + 1 == kb1 || (kb + 1) % (4 * C::kQuads) == 0;
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_mx(d, make_sw128_desc(a0 + kk * 32), make_sw128_desc(b0 + kk * 32), idesc, sf,
-                      sf + 4, (kb > kb0 || kk > 0) ? 1u : 0u);
-          tc_commit(&empty[stage]);
-          if (kb + 1 == kb1 || ((kb + 1) & 3) == 0) {
-            tc_commit(&sempty[slot]);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_mx(d, a0 + 2 * kk, b0 + 2 * kk, idesc, sf, sf + 4,
+                        (kb > kb0 || kk > 0) ? 1u : 0u);
+            tc_commit(&empty[stage]);
+            if (slot_end) tc_commit(&sempty[slot]);
+          }
+          __syncwarp();
+          if (slot_end) {
             if (++slot == SLOTS) {
               slot = 0;
               sphase ^= 1u;
@@ -372,12 +478,14 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
           }
         } else {
           constexpr uint32_t idesc = make_idesc(1u, 0u, kLanes, BN);
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma<kKindF8>(d, make_sw128_desc(a0 + kk * 32), make_sw128_desc(b0 + kk * 32),
-                            idesc, kk > 0 ? 1u : 0u);
-          tc_commit(&empty[stage]);
-          tc_commit(&tfull[buf]);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma<kKindF8>(d, a0 + 2 * kk, b0 + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+            tc_commit(&empty[stage]);
+            tc_commit(&tfull[buf]);
+          }
+          __syncwarp();
           if (++buf == NB) {
             buf = 0;
             bphase ^= 1u;
@@ -390,14 +498,15 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
       }
       if (!ok) break;
       if constexpr (MX) {
-        tc_commit(&tfull[buf]);
+        if (leader) tc_commit(&tfull[buf]);
+        __syncwarp();
         if (++buf == NB) {
           buf = 0;
           bphase ^= 1u;
         }
       }
     }
-    tc_commit(final_bar);
+    if (leader) tc_commit(final_bar);
     volatile int no_abort = 0;
     mbar_wait_bounded(final_bar, 0, &no_abort, limit);
   } else if (warp == 2) {
@@ -405,42 +514,51 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     int slot = 0;
     uint32_t sphase = 0;
     bool ok = true;
-    for (int i = first; ok && i < tiles; i += step) {
-      const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
-      if constexpr (MX) {
-        const uint8_t* xs = static_cast<const uint8_t*>(p.xs);
-        const uint8_t* ws = static_cast<const uint8_t*>(p.ws) + int64_t(tile.n) * p.kb_total;
-        const bool words = p.xs_blk == 1 && p.xs_row % 4 == 0 &&
-                           (reinterpret_cast<uintptr_t>(xs) & 3) == 0;
-        for (int q = kb0 / 4; 4 * q < kb1; ++q) {
-          // loads first, so that they are under way while the slot drains
-          const uint32_t w = scale_word(ws, 1, q, p.kb_total, false);
-          uint32_t v[C::kSfb][4];
+    if constexpr (MX) {
+      constexpr int Q = C::kQuads;
+      const uint8_t* xs = static_cast<const uint8_t*>(p.xs);
+      const bool words = p.xs_blk == 1 && p.xs_row % 4 == 0 &&
+                         (reinterpret_cast<uintptr_t>(xs) & 3) == 0;
+      const int q_first = kb0 / 4 / Q * Q, q_end = (kb1 + 3) / 4;
+      ScaleWords<Q> xw[C::kSfb];
+      BlockWords<Q> ww;
+      auto fetch = [&](int i, int q0) {
+        const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
 #pragma unroll
-          for (int c = 0; c < C::kSfb; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int64_t t = int64_t(tile.t) * BN + 128 * c + 32 * r + lane;
-              const bool in = 128 * c + 32 * r < BN && t < p.T;
-              v[c][r] = in ? scale_word(xs + t * p.xs_row, p.xs_blk, q, p.kb_total, words) : 0u;
-            }
-          ok = mbar_wait_bounded(&sempty[slot], sphase ^ 1u, abort_flag, limit);
-          ok = __all_sync(0xffffffffu, ok);
+        for (int c = 0; c < C::kSfb; ++c) {
+          const int64_t t0 = int64_t(tile.t) * BN + 128 * c;
+          xw[c].fetch(xs, p.xs_row, p.xs_blk, words, t0, min(p.T, t0 + BN), lane, q0, p.kb_total);
+        }
+        ww.fetch(static_cast<const uint8_t*>(p.ws) + int64_t(tile.n) * p.kb_total, true, lane, q0,
+                 p.kb_total);
+      };
+      if (first < tiles) fetch(first, q_first);
+      for (int i = first; ok && i < tiles; i += step) {
+        for (int q0 = q_first; q0 < q_end; q0 += Q) {
+          ok = all_ok(mbar_wait_bounded(&sempty[slot], sphase ^ 1u, abort_flag, limit));
           if (!ok) break;
-          uint4* dst = reinterpret_cast<uint4*>(sRing + slot * 512 * (1 + C::kSfb));
-          dst[lane] = make_uint4(w, w, w, w);
+          uint8_t* dst = sRing + slot * Q * C::kQuadBytes;
+          ww.store(dst, C::kQuadBytes, lane);
 #pragma unroll
-          for (int c = 0; c < C::kSfb; ++c)
-            dst[32 * (1 + c) + lane] = make_uint4(v[c][0], v[c][1], v[c][2], v[c][3]);
+          for (int c = 0; c < C::kSfb; ++c) xw[c].store(dst + 512 * (1 + c), C::kQuadBytes, lane);
           // the copies to tensor memory read it through the async proxy
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          mbar_arrive(&sfull[slot]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfull[slot]);
+          // the next words' loads run while the slots ahead are used
+          if (q0 + Q < q_end)
+            fetch(i, q0 + Q);
+          else if (i + step < tiles)
+            fetch(i + step, q_first);
           if (++slot == SLOTS) {
             slot = 0;
             sphase ^= 1u;
           }
         }
-      } else {
+      }
+    } else {
+      for (int i = first; ok && i < tiles; i += step) {
+        const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
         const float* xs = static_cast<const float*>(p.xs);
         const float* ws = static_cast<const float*>(p.ws) + int64_t(tile.n) * p.kb_total;
         constexpr int R = (BN + 31) / 32;
@@ -459,7 +577,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (32 * r + lane < BN) dst[32 * r + lane] = v[r] * w;
-          mbar_arrive(&sfull[slot]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfull[slot]);
           if (++slot == SLOTS) {
             slot = 0;
             sphase ^= 1u;
@@ -470,7 +589,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   } else if (warp >= 4) {
     // ---------------- promotion and epilogue ----------------
     const int row = (warp & 3) * 32 + lane;
-    const int col0 = ((warp - 4) >> 2) * COLS;
+    const int group = (warp - 4) >> 2;
+    const int col0 = group * COLS;
     const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(col0);
     int buf = 0, slot = 0;
     uint32_t bphase = 0, sphase = 0;
@@ -478,8 +598,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     for (int i = first; epi_ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
       if constexpr (MX) {
-        bool ok = mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit);
-        epi_ok = __all_sync(0xffffffffu, ok);
+        epi_ok = group_ok(1 + group, mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit));
         if (!epi_ok) break;
         tc_fence_after();
         const uint32_t base = lane_base + uint32_t(buf * BN);
@@ -548,10 +667,11 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
             sphase ^= 1u;
           }
         }
+        epi_ok = group_ok(1 + group, epi_ok);
         if (!epi_ok) break;
       }
       if (p.splits == 1) {
-        store_tile(tile, col0, row, (warp - 4) >> 2);
+        store_tile(tile, col0, row, group);
       } else {
         // every MMA of this CTA's only tile has completed, so the stages are
         // free; [token][weight row], a warp writes 32 neighbouring words
@@ -600,26 +720,123 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
 }
 
 // ---------------------------------------------------------------------------
-// fp8_rows_kernel: fp32 scales, 128 tokens x 256 weight rows per tile
+// fp8_pair_kernel: a pair of CTAs (cta_group::2) per tile of 256 tokens x 256
+// weight rows. CTA r of the pair holds tokens 128 r .. (its TMEM lanes) and
+// loads weight rows 128 r .. of the tile; the even CTA issues the MMAs, which
+// read both halves of the weights for both CTAs. Per k-block a CTA takes in
+// and feeds 32 KB instead of the 48 KB of a 128 x 256 tile of its own, which
+// needs 768 cycles of shared-memory bandwidth for the MMA's 512.
 // ---------------------------------------------------------------------------
-struct RowsCfg {
+template <bool MX>
+struct PairCfg {
   static constexpr int kBN = 256;
   static constexpr int kEpiWarps = 16;
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
-  static constexpr int kCols = kBN / (kEpiWarps / 4);  // 64
-  static constexpr int kBBytes = kBN * kKB;
+  static constexpr int kCols = kBN / (kEpiWarps / 4);  // 64 per epilogue warp
+  static constexpr int kBBytes = kBN / 2 * kKB;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 4;
-  static constexpr size_t kSmem = 1024 + 256 + size_t(kStages) * kStageBytes;
-  static constexpr int kBufs = 2;
+  static constexpr int kStages = 6;
+  static constexpr int kSfbChunks = kBN / 128;
+  static constexpr int kSfSlots = 2, kQuads = 4;  // scale ring: slots, quads in each
+  static constexpr int kQuadBytes = 512 * (1 + kSfbChunks);
+  static constexpr int kRingBytes = MX ? kSfSlots * kQuads * kQuadBytes : 0;
+  static constexpr size_t kSmem = 1024 + 512 + kRingBytes + size_t(kStages) * kStageBytes;
+  // TMEM: one accumulator and the scale slots (UE8M0), or two k-block buffers
+  static constexpr int kBufs = MX ? 1 : 2;
+  static constexpr int kSfCol0 = kBufs * kBN;
+  static constexpr int kSfCols = 4 * (1 + kSfbChunks);
+  static_assert(kSfCol0 + (MX ? kSfSlots * kQuads * kSfCols : 0) <= 512, "TMEM columns");
+  static_assert(8 * (2 * kStages + 2 * kSfSlots + 2 * kBufs + 1) + 8 <= 512, "barriers");
   // The block launches at kLaunchRegs registers per thread; the control
   // warpgroup gives registers back and the 16 epilogue warps take them, for 64
   // sums and a batch of 32 partials each. The split adds up to the launch's
   // total, which the host checks against the compiled kernel.
-  static constexpr int kLaunchRegs = 96, kCtrlRegs = 32, kEpiRegs = 112;
+  static constexpr int kLaunchRegs = 96, kCtrlRegs = 64, kEpiRegs = 104;
   static_assert(128 * kCtrlRegs + 32 * kEpiWarps * kEpiRegs == kThreads * kLaunchRegs,
                 "setmaxnreg split");
 };
+
+// Shared-memory address `addr` of this CTA in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+// Arrives on a barrier of the cluster, after this thread's (and, after a warp
+// barrier, its warp's) writes.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+// The same where no memory is handed over but tensor memory that has been
+// read: the cluster-wide release would wait for unrelated loads and stores.
+__device__ __forceinline__ void mbar_arrive_cluster_read(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// mbar_wait_bounded for a phase that threads of the other CTA complete too.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "n"(kMbarSuspendHintNs)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
+                                                  volatile int* abort, uint64_t limit_ns) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > limit_ns) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+// TMA load into this CTA whose bytes are counted on the even CTA's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* tm, int32_t c0,
+                                              int32_t c1, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(leader_bar)
+      : "memory");
+}
+// Arrives on `bar` of both CTAs when the MMAs issued so far have completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+// Scale chunk at the same shared-memory offset of each CTA into its own TMEM.
+__device__ __forceinline__ void tc_cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
+               : "memory");
+}
 
 // Transposes 4 x 4 vectors among the lanes of a quad: lane i's vector c
 // becomes lane c's vector i (its own inverse).
@@ -653,11 +870,11 @@ __device__ __forceinline__ uint4 pack16(const float* x) {
                       pack2<T>(x[6], x[7]));
 }
 
-template <typename TOUT>
-__global__ void __launch_bounds__(RowsCfg::kThreads, 1)
-    fp8_rows_kernel(const __grid_constant__ CUtensorMap tmX,
+template <bool MX, typename TOUT>
+__global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap tmX,
                     const __grid_constant__ CUtensorMap tmW, const MatmulParams p) {
-  using C = RowsCfg;
+  using C = PairCfg<MX>;
   constexpr int STAGES = C::kStages;
   constexpr int NB = C::kBufs;
   constexpr int COLS = C::kCols;
@@ -667,35 +884,48 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + STAGES * kABytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sB + STAGES * C::kBBytes);
+  uint8_t* sRing = sB + STAGES * C::kBBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sRing + C::kRingBytes);  // used in the even CTA
   uint64_t* empty = full + STAGES;
-  uint64_t* tfull = empty + STAGES;
-  uint64_t* tempty = tfull + NB;
+  uint64_t* sfull = empty + STAGES;  // used in the even CTA
+  uint64_t* sempty = sfull + C::kSfSlots;
+  uint64_t* tfull = sempty + C::kSfSlots;
+  uint64_t* tempty = tfull + NB;  // used in the even CTA
   uint64_t* final_bar = tempty + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5;
+  // the warp's number, known to be the same for all its lanes
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = blockIdx.x & 1;  // in the pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < C::kSfSlots; ++s) {
+      mbar_init(&sfull[s], 2);
+      mbar_init(&sempty[s], 1);
+    }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], C::kEpiWarps);
+      mbar_init(&tempty[b], 2 * C::kEpiWarps);
     }
     mbar_init(final_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  cluster_sync();  // both CTAs' barriers and TMEM are ready
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
@@ -703,178 +933,318 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
   const uint64_t limit = p.wait_limit_ns;
   const int tiles = p.t_tiles * p.n_tiles;
   const int kbs = p.kb_total;
+  const int first = int(blockIdx.x) >> 1, step = int(gridDim.x) >> 1;
 
-  if (warp < 4) setmaxnreg_dec<C::kCtrlRegs>();
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmX);
-    tma_prefetch_desc(&tmW);
-    int stage = 0;
-    uint32_t phase = 0, issued = 0;
+  if (!MX && warp < 4) setmaxnreg_dec<C::kCtrlRegs>();
+  if (producer_of(warp) >= 0) {
+    // ---------------- TMA producers of this CTA's halves ----------------
+    const bool leader = elect_one();
+    if (leader) {
+      tma_prefetch_desc(&tmX);
+      tma_prefetch_desc(&tmW);
+    }
+    const int mine = producer_of(warp);
+    const uint32_t bars = peer_addr(smem_u32(full), 0);  // the even CTA's
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    Filled filled;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+    for (int i = first; ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
+      const int x_row = tile.t * 256 + int(rank) * kLanes;
+      const int w_row = tile.n * C::kBN + int(rank) * (C::kBN / 2);
       for (int kb = 0; kb < kbs; ++kb) {
-        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, limit)) {
-          ok = false;
-          break;
+        if (turn == mine) {
+          ok = all_ok(mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, limit));
+          if (!ok) break;
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
+            const uint32_t bar = bars + 8u * uint32_t(stage);
+            tma_load_pair(sA + stage * kABytes, &tmX, kb * kKB, x_row, bar);
+            tma_load_pair(sB + stage * C::kBBytes, &tmW, kb * kKB, w_row, bar);
+          }
+          __syncwarp();
         }
-        mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
-        tma_load_2d(sA + stage * kABytes, &tmX, kb * kKB, tile.t * kLanes, &full[stage]);
-        tma_load_2d(sB + stage * C::kBBytes, &tmW, kb * kKB, tile.n * C::kBN, &full[stage]);
-        ++issued;
+        filled.add(stage, phase);
+        turn = turn + 1 == kProducers ? 0 : turn + 1;
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    drain_ring(full, STAGES, issued, limit);
-  } else if (warp == 1 && lane == 0) {
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, bphase = 0;
+    // the even CTA's barriers count both CTAs' bytes; the odd CTA stays until
+    // the cluster barrier below
+    if (rank == 0) filled.drain(full, STAGES, limit);
+  } else if (warp == 1 && rank == 0) {
+    // ---------------- MMA issuer, for both CTAs ----------------
+    // The whole warp walks the loop and one lane issues: operands computed by
+    // a converged warp stay in uniform registers, where the MMA takes them.
+    const bool leader = elect_one();
+    const uint64_t desc_a = make_sw128_desc(smem_u32(sA));
+    const uint64_t desc_b = make_sw128_desc(smem_u32(sB));
+    int stage = 0, buf = 0, slot = 0;
+    [[maybe_unused]] uint32_t sf = 0;  // TMEM of the quad's scales
+    uint32_t phase = 0, bphase = 0, sphase = 0;
     bool ok = true;
-    constexpr uint32_t idesc = make_idesc(1u, 0u, kLanes, C::kBN);
-    for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+    for (int i = first; ok && i < tiles; i += step) {
+      if constexpr (MX) {
+        if (!all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit))) break;
+        tc_fence_after();
+      }
       for (int kb = 0; kb < kbs; ++kb) {
-        if (!mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit) ||
-            !mbar_wait_bounded(&full[stage], phase, abort_flag, limit)) {
-          ok = false;
-          break;
+        if constexpr (MX) {
+          if (kb % (4 * C::kQuads) == 0) {
+            ok = all_ok(mbar_wait_cluster(&sfull[slot], sphase, abort_flag, limit));
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if ((kb & 3) == 0) {
+            const int quad = slot * C::kQuads + (kb >> 2) % C::kQuads;
+            sf = tmem_base + uint32_t(C::kSfCol0 + quad * C::kSfCols);
+            const uint32_t src = smem_u32(sRing + quad * C::kQuadBytes);
+            if (leader) {
+#pragma unroll
+              for (int c = 0; c < 1 + C::kSfbChunks; ++c)
+                tc_cp_sf_pair(sf + 4 * c, make_sf_desc(src + 512 * c));
+            }
+            __syncwarp();
+          }
+        } else {
+          ok = all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit));
+          if (!ok) break;
         }
+        ok = all_ok(mbar_wait_bounded(&full[stage], phase, abort_flag, limit));
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem_base + uint32_t(buf * C::kBN);
-        const uint32_t a0 = smem_u32(sA + stage * kABytes);
-        const uint32_t b0 = smem_u32(sB + stage * C::kBBytes);
+        // descriptors of the stage's tiles; 32 bytes further along K are 2 units
+        const uint64_t a0 = desc_a + uint32_t(stage * (kABytes / 16));
+        const uint64_t b0 = desc_b + uint32_t(stage * (C::kBBytes / 16));
+        if constexpr (MX) {
+          const uint32_t idesc = idesc_sf_ids(make_idesc_mx(256, C::kBN), uint32_t(kb & 3));
+          const bool slot_end = kb + 1 == kbs || (kb + 1) % (4 * C::kQuads) == 0;
+          if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc_mma<kKindF8>(d, make_sw128_desc(a0 + kk * 32), make_sw128_desc(b0 + kk * 32), idesc,
-                          kk > 0 ? 1u : 0u);
-        tc_commit(&empty[stage]);
-        tc_commit(&tfull[buf]);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_mx_pair(d, a0 + 2 * kk, b0 + 2 * kk, idesc, sf, sf + 4,
+                             (kb > 0 || kk > 0) ? 1u : 0u);
+            tc_commit_pair(&empty[stage]);
+            if (slot_end) tc_commit_pair(&sempty[slot]);
+          }
+          __syncwarp();
+          if (slot_end) {
+            if (++slot == C::kSfSlots) {
+              slot = 0;
+              sphase ^= 1u;
+            }
+          }
+        } else {
+          constexpr uint32_t idesc = make_idesc(1u, 0u, 256, C::kBN);
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_f8_pair(d, a0 + 2 * kk, b0 + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+            tc_commit_pair(&empty[stage]);
+            tc_commit_pair(&tfull[buf]);
+          }
+          __syncwarp();
+          if (++buf == NB) {
+            buf = 0;
+            bphase ^= 1u;
+          }
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if constexpr (MX) {
+        if (leader) tc_commit_pair(&tfull[buf]);
+        __syncwarp();
         if (++buf == NB) {
           buf = 0;
           bphase ^= 1u;
         }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+      }
+    }
+    if (leader)
+      asm volatile(
+          "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+              smem_u32(final_bar))
+          : "memory");
+    volatile int no_abort = 0;
+    mbar_wait_bounded(final_bar, 0, &no_abort, limit);
+  } else if (MX && warp == 2) {
+    // ---------------- scales: this CTA's tokens, all of the tile's weights ----------------
+    const uint8_t* xs = static_cast<const uint8_t*>(p.xs);
+    const bool words = p.xs_blk == 1 && p.xs_row % 4 == 0 &&
+                       (reinterpret_cast<uintptr_t>(xs) & 3) == 0;
+    const int64_t w_blocks = (p.N + 127) / 128;
+    const int quads = (kbs + 3) / 4;
+    constexpr int Q = C::kQuads;
+    ScaleWords<Q> xw;
+    BlockWords<Q> ww[C::kSfbChunks];
+    auto fetch = [&](int i, int q0) {
+      const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
+      xw.fetch(xs, p.xs_row, p.xs_blk, words, int64_t(tile.t) * 256 + rank * kLanes, p.T, lane, q0,
+               kbs);
+#pragma unroll
+      for (int c = 0; c < C::kSfbChunks; ++c) {
+        const int64_t nb = int64_t(tile.n) * C::kSfbChunks + c;
+        ww[c].fetch(static_cast<const uint8_t*>(p.ws) + nb * kbs, nb < w_blocks, lane, q0, kbs);
+      }
+    };
+    int slot = 0;
+    uint32_t sphase = 0;
+    bool ok = true;
+    if (first < tiles) fetch(first, 0);
+    for (int i = first; ok && i < tiles; i += step) {
+      for (int q0 = 0; q0 < quads; q0 += Q) {
+        ok = all_ok(mbar_wait_bounded(&sempty[slot], sphase ^ 1u, abort_flag, limit));
+        if (!ok) break;
+        uint8_t* dst = sRing + slot * Q * C::kQuadBytes;
+        xw.store(dst, C::kQuadBytes, lane);
+#pragma unroll
+        for (int c = 0; c < C::kSfbChunks; ++c) ww[c].store(dst + 512 * (1 + c), C::kQuadBytes, lane);
+        // the copies to tensor memory read it through the async proxy
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&sfull[slot]), 0));
+        // the next words' loads run while the slots ahead are used
+        if (q0 + Q < quads)
+          fetch(i, q0 + Q);
+        else if (i + step < tiles)
+          fetch(i + step, 0);
+        if (++slot == C::kSfSlots) {
+          slot = 0;
+          sphase ^= 1u;
         }
       }
     }
-    tc_commit(final_bar);
-    volatile int no_abort = 0;
-    mbar_wait_bounded(final_bar, 0, &no_abort, limit);
   } else if (warp >= 4) {
-    setmaxnreg_inc<C::kEpiRegs>();
+    // ---------------- promotion and epilogue of this CTA's 128 tokens ----------------
+    if constexpr (!MX) setmaxnreg_inc<C::kEpiRegs>();
     const int row = (warp & 3) * 32 + lane;
     const int col0 = ((warp - 4) >> 2) * COLS;
     const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(col0);
-    const float* xs = static_cast<const float*>(p.xs);
-    const float* ws = static_cast<const float*>(p.ws);
+    const uint32_t tempty0 = peer_addr(smem_u32(&tempty[0]), 0);
     const int64_t w_blocks = (p.N + 127) / 128;
-    // 16-byte stores when every output row starts on such a boundary
     constexpr int kVec = 16 / int(sizeof(TOUT));
-    const bool vec = p.ld_out % kVec == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-    const bool add_vec = p.ld_add % kVec == 0 && (reinterpret_cast<uintptr_t>(p.add) & 15) == 0;
     int buf = 0;
     uint32_t bphase = 0;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+    for (int i = first; ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
-      const int64_t t = int64_t(tile.t) * kLanes + row;
+      const int64_t t = int64_t(tile.t) * 256 + rank * kLanes + row;
       const int64_t n0 = int64_t(tile.n) * C::kBN + col0;
-      const bool live = t < p.T;
-      const int64_t wb = min(n0 / 128, w_blocks - 1);  // columns past N have no scale
-      const float* sx = xs + (live ? t * p.xs_row : 0);
-      const float* sw = ws + wb * kbs;
       float acc[COLS];
-#pragma unroll
-      for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
-      // the next k-block's scales are on their way while this one is added
-      float sx_n = __ldg(sx), sw_n = __ldg(sw);
-      for (int kb = 0; kb < kbs; ++kb) {
-        float s = sx_n * sw_n;
-        if (kb + 1 < kbs) {
-          sx_n = __ldg(sx + (kb + 1) * p.xs_blk);
-          sw_n = __ldg(sw + kb + 1);
-        }
+      if constexpr (MX) {
         ok = mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t base = lane_base + uint32_t(buf * C::kBN);
+        uint32_t v[COLS];
+        tmem_ld32(lane_base + uint32_t(buf * C::kBN), *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld32(lane_base + uint32_t(buf * C::kBN) + 32,
+                  *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_arrived(v);
 #pragma unroll
-        for (int c = 0; c < COLS; c += BATCH) {
-          uint32_t v[BATCH];
-          tmem_ld32(base + c, v);
-          tmem_ld_wait();
-          asm volatile("" : "+f"(s));  // no product can move before the wait
-          if (c + BATCH >= COLS) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[buf]);
-          }
-#pragma unroll
-          for (int j = 0; j < BATCH; ++j)
-            acc[c + j] = fmaf(s, __uint_as_float(v[j]), acc[c + j]);
-        }
+        for (int j = 0; j < COLS; ++j) acc[j] = __uint_as_float(v[j]);
+        // the tile is in registers: the next one's MMAs may start
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_read(tempty0 + 8 * buf);
         if (++buf == NB) {
           buf = 0;
           bphase ^= 1u;
         }
+      } else {
+        const int64_t wb = min(n0 / 128, w_blocks - 1);  // columns past N have no scale
+        const float* sx = static_cast<const float*>(p.xs) + (t < p.T ? t * p.xs_row : 0);
+        const float* sw = static_cast<const float*>(p.ws) + wb * kbs;
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
+        // the next k-block's scales are on their way while this one is added
+        float sx_n = __ldg(sx), sw_n = __ldg(sw);
+        for (int kb = 0; kb < kbs; ++kb) {
+          float s = sx_n * sw_n;
+          if (kb + 1 < kbs) {
+            sx_n = __ldg(sx + (kb + 1) * p.xs_blk);
+            sw_n = __ldg(sw + kb + 1);
+          }
+          ok = mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t base = lane_base + uint32_t(buf * C::kBN);
+#pragma unroll
+          for (int c = 0; c < COLS; c += BATCH) {
+            uint32_t v[BATCH];
+            tmem_ld32(base + c, v);
+            tmem_ld_wait();
+            asm volatile("" : "+f"(s));  // no product can move before the wait
+            if (c + BATCH >= COLS) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster_read(tempty0 + 8 * buf);
+            }
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+              acc[c + j] = fmaf(s, __uint_as_float(v[j]), acc[c + j]);
+          }
+          if (++buf == NB) {
+            buf = 0;
+            bphase ^= 1u;
+          }
+        }
+        if (!ok) break;
       }
-      if (!ok) continue;
+      // N is a multiple of kVec here. A quad of lanes trades vectors so that
+      // it stores 64 bytes of one row at a time (and reads the addend so).
       TOUT* out = static_cast<TOUT*>(p.out) + n0;
       const TOUT* add = static_cast<const TOUT*>(p.add) + n0;
-      const int cols = int(min(int64_t(COLS), max(int64_t(0), p.N - n0)));
-      if (vec && cols == COLS && (p.add == nullptr || add_vec)) {
-        // a quad of lanes trades vectors so that it stores 64 bytes of one
-        // row at a time (and reads the addend so)
-        const int64_t t4 = t - (lane & 3);
-        const int mine = (lane & 3) * kVec;
+      const int64_t t4 = t - (lane & 3);
+      const int mine = (lane & 3) * kVec;
 #pragma unroll
-        for (int j = 0; j < COLS; j += 4 * kVec) {
-          uint4 v[4];
-          if (p.add != nullptr) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              v[r] = t4 + r < p.T ? *reinterpret_cast<const uint4*>(add + (t4 + r) * p.ld_add +
-                                                                    j + mine)
-                                  : make_uint4(0, 0, 0, 0);
-            quad_transpose(v, lane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const TOUT* e = reinterpret_cast<const TOUT*>(&v[r]);
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) acc[j + r * kVec + k] += to_f32(e[k]);
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = pack16<TOUT>(&acc[j + r * kVec]);
-          quad_transpose(v, lane);
+      for (int j = 0; j < COLS; j += 4 * kVec) {
+        const bool in = n0 + j + mine < p.N;
+        uint4 v[4];
+        if (p.add != nullptr) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (t4 + r < p.T)
-              *reinterpret_cast<uint4*>(out + (t4 + r) * p.ld_out + j + mine) = v[r];
-        }
-      } else if (live) {
-        out += t * p.ld_out;
-        add += t * p.ld_add;
+            v[r] = in && t4 + r < p.T
+                       ? *reinterpret_cast<const uint4*>(add + (t4 + r) * p.ld_add + j + mine)
+                       : make_uint4(0, 0, 0, 0);
+          quad_transpose(v, lane);
 #pragma unroll
-        for (int j = 0; j < COLS; ++j)
-          if (j < cols) {
-            if (p.add != nullptr) acc[j] += to_f32(add[j]);
-            out[j] = from_f32<TOUT>(acc[j]);
+          for (int r = 0; r < 4; ++r) {
+            const TOUT* e = reinterpret_cast<const TOUT*>(&v[r]);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) acc[j + r * kVec + k] += to_f32(e[k]);
           }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = pack16<TOUT>(&acc[j + r * kVec]);
+        quad_transpose(v, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (in && t4 + r < p.T)
+            *reinterpret_cast<uint4*>(out + (t4 + r) * p.ld_out + j + mine) = v[r];
       }
     }
   }
+  tc_fence_before();
   __syncwarp();
   __syncthreads();
+  cluster_sync();  // the even CTA's MMAs read both CTAs' memory until here
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(512)
+                 : "memory");
   }
   if (threadIdx.x == 0 && *abort_flag) report_status(p.status, MOE_ERR_TIMEOUT);
 }
@@ -883,19 +1253,17 @@ __global__ void __launch_bounds__(RowsCfg::kThreads, 1)
 // Host side
 // ---------------------------------------------------------------------------
 struct Plan {
-  int rows;    // 1: fp8_rows_kernel
-  int bn;      // columns per tile (tokens; weight rows for fp8_rows_kernel)
+  int pair;    // 1: fp8_pair_kernel
+  int bn;      // columns per tile (tokens; weight rows for fp8_pair_kernel)
   int splits;  // CTAs per cluster along K
   int ctas;
 };
 
-Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
+// `vec`: the output's rows (and the addend's) start on 16-byte boundaries,
+// as the pair kernel's stores need.
+Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, bool vec, int sms) {
   const int64_t kbs = ceil_div(K, kKB);
   Plan best = {0, 16, 1, 1};
-  if (!mx && T > 128) {
-    const int64_t tiles = ceil_div(T, kLanes) * ceil_div(N, 256);
-    return {1, 256, 1, int(std::min<int64_t>(tiles, sms))};
-  }
   double best_cost = 1e300;
   for (int bn : {16, 32, 64, 128, 256}) {
     if (bn == 256 && !mx) continue;
@@ -905,8 +1273,10 @@ Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
       const int occ = bn <= 64 ? 2 : 1;
       if (s > 1 && tiles * s > int64_t(sms) * occ) break;
       // cycles: k-blocks one after another on an SM, each the MMA's or, when
-      // longer, its share of the bytes an SM takes in; then a tile's epilogue
-      const double per_kb = std::max(2.0 * bn, (kABytes + bn * kKB) / 56.0);
+      // longer, its share of the bytes an SM takes in (and, for fp32 scales,
+      // the promotion of its columns); then a tile's epilogue
+      double per_kb = std::max(3.0 * bn, (kABytes + bn * kKB) / 56.0);
+      if (!mx) per_kb = std::max(per_kb, 200 + 3.0 * bn);
       const double per_tile = 400 + 4.0 * bn;
       const double waves = double(ceil_div(tiles * s, sms));
       const double cost = waves * (double(ceil_div(kbs, s)) * per_kb + per_tile) +
@@ -917,6 +1287,12 @@ Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
                 int(s > 1 ? tiles * s : std::min<int64_t>(tiles, int64_t(sms) * occ))};
       }
     }
+  }
+  if (vec && T > 128) {
+    const int64_t tiles = ceil_div(T, 256) * ceil_div(N, 256);
+    const double waves = double(ceil_div(tiles, sms / 2));
+    const double cost = waves * (kbs * (mx ? 540.0 : 620.0) + (mx ? 1000 : 600)) + 1500;
+    if (cost < best_cost) best = {1, 256, 1, int(2 * std::min<int64_t>(tiles, sms / 2))};
   }
   return best;
 }
@@ -982,24 +1358,31 @@ int dispatch_cols(const Plan& plan, const CUtensorMap& w, const CUtensorMap& x,
   return fail(MOE_ERR_UNSUPPORTED, "fp8_matmul: no such tile");
 }
 
+template <bool MX, typename TOUT>
+int launch_pair(const Plan& plan, const CUtensorMap& w, const CUtensorMap& x,
+                const MatmulParams& p, cudaStream_t s) {
+  using C = PairCfg<MX>;
+  static std::atomic<uint64_t> done{0};
+  int st = set_smem_once(fp8_pair_kernel<MX, TOUT>, C::kSmem, done);
+  if (st != MOE_OK) return st;
+  // a register split that the launch cannot cover would never return
+  static const int regs = [] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, fp8_pair_kernel<MX, TOUT>) == cudaSuccess ? attr.numRegs
+                                                                                  : -1;
+  }();
+  KSW_REQUIRE(MX || regs == C::kLaunchRegs, MOE_ERR_UNSUPPORTED,
+              "fp8_matmul: compiled register count does not match the setmaxnreg split");
+  return launch_clusters(fp8_pair_kernel<MX, TOUT>, plan.ctas, C::kThreads, C::kSmem, 2, s, x, w,
+                         p);
+}
+
 template <typename TOUT>
 int run_matmul(const Plan& plan, bool mx, const CUtensorMap& w, const CUtensorMap& x,
                const MatmulParams& p, cudaStream_t s) {
-  if (plan.rows) {
-    static std::atomic<uint64_t> done{0};
-    int st = set_smem_once(fp8_rows_kernel<TOUT>, RowsCfg::kSmem, done);
-    if (st != MOE_OK) return st;
-    // a register split that the launch cannot cover would never return
-    static const int regs = [] {
-      cudaFuncAttributes attr;
-      return cudaFuncGetAttributes(&attr, fp8_rows_kernel<TOUT>) == cudaSuccess ? attr.numRegs
-                                                                                : -1;
-    }();
-    KSW_REQUIRE(regs == RowsCfg::kLaunchRegs, MOE_ERR_UNSUPPORTED,
-                "fp8_matmul: compiled register count does not match the setmaxnreg split");
-    return launch_clusters(fp8_rows_kernel<TOUT>, plan.ctas, RowsCfg::kThreads, RowsCfg::kSmem, 1,
-                           s, x, w, p);
-  }
+  if (plan.pair)
+    return mx ? launch_pair<true, TOUT>(plan, w, x, p, s)
+              : launch_pair<false, TOUT>(plan, w, x, p, s);
   return mx ? dispatch_cols<true, TOUT>(plan, w, x, p, s)
             : dispatch_cols<false, TOUT>(plan, w, x, p, s);
 }
@@ -1025,8 +1408,9 @@ extern "C" int moe_fp8_matmul_plan(int64_t num_rows, int64_t out_cols, int64_t i
   int st = check_sizes(num_rows, out_cols, inner, scale_format);
   if (st != MOE_OK) return st;
   KSW_REQUIRE(info != nullptr, MOE_ERR_INVALID_ARG, "fp8_matmul_plan: null pointer");
-  const Plan plan = plan_matmul(num_rows, out_cols, inner, scale_format == 1, 148);
-  info[0] = plan.rows;
+  const Plan plan =
+      plan_matmul(num_rows, out_cols, inner, scale_format == 1, out_cols % 8 == 0, 148);
+  info[0] = plan.pair;
   info[1] = plan.bn;
   info[2] = plan.splits;
   info[3] = num_rows == 0 ? 0 : plan.ctas;
@@ -1057,15 +1441,17 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   KSW_REQUIRE(x && x_scale && w && w_scale && out, MOE_ERR_INVALID_ARG,
               "fp8_matmul: null pointer");
   const bool mx = scale_format == 1;
-  const Plan plan = plan_matmul(num_rows, out_cols, inner, mx, sms);
+  const int vec = out_dtype == MOE_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  const bool aligned = out_cols % vec == 0 && ld_out % vec == 0 && aligned16(out) &&
+                       (addend == nullptr || (ld_addend % vec == 0 && aligned16(addend)));
+  const Plan plan = plan_matmul(num_rows, out_cols, inner, mx, aligned, sms);
   CUtensorMap tx, tw;
-  const uint32_t x_box = plan.rows ? kLanes : uint32_t(plan.bn);
-  const uint32_t w_box = plan.rows ? uint32_t(plan.bn) : kLanes;
+  const uint32_t x_box = plan.pair ? kLanes : uint32_t(plan.bn);
   st = encode_tma_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, uint64_t(inner),
                      uint64_t(num_rows), uint64_t(ld_x), kKB, x_box);
   if (st != MOE_OK) return st;
   st = encode_tma_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, uint64_t(inner),
-                     uint64_t(out_cols), uint64_t(ld_w), kKB, w_box);
+                     uint64_t(out_cols), uint64_t(ld_w), kKB, kLanes);
   if (st != MOE_OK) return st;
   MatmulParams p = {};
   p.xs = x_scale;
@@ -1079,8 +1465,8 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   p.T = num_rows;
   p.N = out_cols;
   p.kb_total = int(ceil_div(inner, kKB));
-  p.t_tiles = int(ceil_div(num_rows, plan.rows ? kLanes : plan.bn));
-  p.n_tiles = int(ceil_div(out_cols, plan.rows ? plan.bn : kLanes));
+  p.t_tiles = int(ceil_div(num_rows, plan.pair ? 256 : plan.bn));
+  p.n_tiles = int(ceil_div(out_cols, plan.pair ? plan.bn : kLanes));
   p.splits = plan.splits;
   p.status = status;
   p.wait_limit_ns = kWaitLimitNs;

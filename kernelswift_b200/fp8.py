@@ -182,7 +182,7 @@ def block_matmul_plan(num_rows: int, out_cols: int, inner: int, scale_format: st
 
     info = (ctypes.c_int32 * 4)()
     _lib.call("moe_fp8_matmul_plan", num_rows, out_cols, inner, _FORMAT[scale_format], info)
-    return dict(zip(("tokens_on_rows", "tile_cols", "splits", "ctas"), list(info)))
+    return dict(zip(("cta_pairs", "tile_cols", "splits", "ctas"), list(info)))
 
 
 def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,

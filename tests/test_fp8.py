@@ -64,8 +64,8 @@ def test_plan_covers_the_product(fmt):
                 kb = -(-K // 128)
                 assert 1 <= p["splits"] <= min(8, kb)
                 assert p["tile_cols"] in (16, 32, 64, 128, 256)
-                if p["tokens_on_rows"]:
-                    tiles = -(-T // 128) * -(-N // p["tile_cols"])
+                if p["cta_pairs"]:
+                    tiles = 2 * (-(-T // 256) * -(-N // 256))
                 else:
                     tiles = -(-T // p["tile_cols"]) * -(-N // 128)
                 if p["splits"] > 1:

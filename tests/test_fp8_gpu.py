@@ -187,7 +187,7 @@ def check_product(out, x, w, addend=None):
 SIZES = [(1, 1, 1), (1, 128, 128), (3, 17, 100), (16, 130, 129), (17, 256, 640), (31, 300, 1000),
          (33, 129, 2000), (64, 576, 512), (65, 384, 300), (100, 77, 4000), (128, 640, 1536),
          (129, 257, 130), (200, 1024, 1000), (257, 513, 999), (333, 1500, 1000), (600, 2049, 256),
-         (1, 4096, 7168), (5, 7168, 2048)]
+         (1, 4096, 7168), (5, 7168, 2048), (513, 1032, 2000), (1000, 4104, 384), (2049, 1544, 700)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -206,7 +206,7 @@ def test_product(cuda_device, T, N, K, fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_large_products_by_rows(cuda_device, fmt):
     """Many tiles per CTA: rows drawn from a product too large for the oracle."""
-    T, N, K = 3000, 4100, 1100
+    T, N, K = 5000, 4104, 1100
     x, w = operands(T, N, K, fmt, cuda_device)
     out = fp8.block_matmul(*x, *w)
     rows = torch.cat([torch.arange(0, T, 37), torch.tensor([T - 1])])
