@@ -149,34 +149,43 @@ __device__ __forceinline__ int producer_of(int warp) { return warp == 0 ? 0 : wa
 
 // UE8M0 scales travel as words of four bytes, the scales of one row in a quad
 // of k-blocks. A loader warp builds the tensor core's 512-byte chunks (128
-// rows: lane l holds rows l, l + 32, l + 64, l + 96) of Q quads at a time:
-// some 16 loads under way per lane instead of four, since a turn of the loader
-// takes 2,000 to 3,600 cycles and a quad's MMAs only 2,048.
+// rows: lane l holds rows l, l + 32, l + 64, l + 96) of Q quads at a time.
 template <int Q>
 struct ScaleWords {
   uint32_t v[4][Q];
 
-  // The words of quads q0 .. q0 + Q of 128 rows of `scale` from row `row0`, of
-  // which those below `rows` exist; bytes past the KB blocks are 0.
+  // The words of quads q0 .. q0 + Q of the 128 rows of `scale` from row0 on.
+  // Rows at or past `rows` and quads past the last repeat the last one (their
+  // products are never stored, or never made), so that all loads are
+  // unconditional and under way together: loaded one by one behind branches
+  // they took 2,000 to 3,600 cycles a quad, and a quad's MMAs take 2,048.
   __device__ __forceinline__ void fetch(const uint8_t* scale, int64_t row_stride,
                                         int64_t blk_stride, bool words, int64_t row0,
                                         int64_t rows, int lane, int q0, int kb) {
+    const uint8_t* at[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t t = row0 + 32 * r + lane;
-      const uint8_t* at = scale + t * row_stride;
+    for (int r = 0; r < 4; ++r)
+      at[r] = scale + min(row0 + 32 * r + lane, rows - 1) * row_stride;
+    if (words) {
+      const int last = kb / 4 - 1;  // whole words
 #pragma unroll
-      for (int j = 0; j < Q; ++j) {
-        const int b = 4 * (q0 + j);
-        v[r][j] = 0;
-        if (t < rows) {
-          if (words && b + 4 <= kb) {
-            v[r][j] = __ldg(reinterpret_cast<const uint32_t*>(at + b));
-          } else {
+      for (int j = 0; j < Q; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (b + i < kb) v[r][j] |= uint32_t(__ldg(at + (b + i) * blk_stride)) << (8 * i);
-          }
+        for (int r = 0; r < 4; ++r)
+          v[r][j] = __ldg(reinterpret_cast<const uint32_t*>(at[r]) + min(q0 + j, last));
+    }
+    // quads with fewer than four blocks, and scales that are not in words
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+      const int b = 4 * (q0 + j);
+      if (b < kb && (!words || b + 4 > kb)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w |= uint32_t(__ldg(at[r] + min(b + i, kb - 1) * blk_stride)) << (8 * i);
+          v[r][j] = w;
         }
       }
     }
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     if constexpr (MX) {
       constexpr int Q = C::kQuads;
       const uint8_t* xs = static_cast<const uint8_t*>(p.xs);
-      const bool words = p.xs_blk == 1 && p.xs_row % 4 == 0 &&
+      const bool words = p.kb_total >= 4 && p.xs_blk == 1 && p.xs_row % 4 == 0 &&
                          (reinterpret_cast<uintptr_t>(xs) & 3) == 0;
       const int q_first = kb0 / 4 / Q * Q, q_end = (kb1 + 3) / 4;
       ScaleWords<Q> xw[C::kSfb];
@@ -730,9 +739,15 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
 template <bool MX>
 struct PairCfg {
   static constexpr int kBN = 256;
-  static constexpr int kEpiWarps = 16;
+  static constexpr int kEpiWarps = MX ? 16 : 8;
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
-  static constexpr int kCols = kBN / (kEpiWarps / 4);  // 64 per epilogue warp
+  static constexpr int kCols = kBN / (kEpiWarps / 4);  // per epilogue warp: 64 or 128
+  // fp32 scales: a k-block's product is two MMAs of 128 columns, each with its
+  // own issuing warp, buffers and barriers, so that four buffers of 128 columns
+  // hide the way from an MMA's end to its buffer's release
+  static constexpr int kHalves = MX ? 1 : 2;
+  static constexpr int kN = kBN / kHalves;             // columns of an MMA
+  static constexpr int kBox = kN / 2;                  // weight rows of a CTA's TMA box
   static constexpr int kBBytes = kBN / 2 * kKB;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 6;
@@ -746,13 +761,14 @@ struct PairCfg {
   static constexpr int kSfCol0 = kBufs * kBN;
   static constexpr int kSfCols = 4 * (1 + kSfbChunks);
   static_assert(kSfCol0 + (MX ? kSfSlots * kQuads * kSfCols : 0) <= 512, "TMEM columns");
-  static_assert(8 * (2 * kStages + 2 * kSfSlots + 2 * kBufs + 1) + 8 <= 512, "barriers");
-  // The block launches at kLaunchRegs registers per thread; the control
-  // warpgroup gives registers back and the 16 epilogue warps take them, for 64
-  // sums and a batch of 32 partials each. The split adds up to the launch's
-  // total, which the host checks against the compiled kernel.
-  static constexpr int kLaunchRegs = 96, kCtrlRegs = 64, kEpiRegs = 104;
-  static_assert(128 * kCtrlRegs + 32 * kEpiWarps * kEpiRegs == kThreads * kLaunchRegs,
+  static_assert(8 * (2 * kStages + 2 * kSfSlots + 2 * kBufs * kHalves + 1) + 8 <= 512,
+                "barriers");
+  // fp32 scales: the block launches at kLaunchRegs registers per thread; the
+  // control warpgroup gives registers back and the 8 epilogue warps take them,
+  // for 128 sums and a batch of 64 partials each. The split adds up to the
+  // launch's total, which the host checks against the compiled kernel.
+  static constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kEpiRegs = 216;
+  static_assert(MX || 128 * kCtrlRegs + 32 * kEpiWarps * kEpiRegs == kThreads * kLaunchRegs,
                 "setmaxnreg split");
 };
 
@@ -878,7 +894,6 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
   constexpr int STAGES = C::kStages;
   constexpr int NB = C::kBufs;
   constexpr int COLS = C::kCols;
-  constexpr int BATCH = 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -890,8 +905,8 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
   uint64_t* sfull = empty + STAGES;  // used in the even CTA
   uint64_t* sempty = sfull + C::kSfSlots;
   uint64_t* tfull = sempty + C::kSfSlots;
-  uint64_t* tempty = tfull + NB;  // used in the even CTA
-  uint64_t* final_bar = tempty + NB;
+  uint64_t* tempty = tfull + NB * C::kHalves;  // used in the even CTA
+  uint64_t* final_bar = tempty + NB * C::kHalves;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -902,17 +917,17 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], C::kHalves);
     }
     for (int s = 0; s < C::kSfSlots; ++s) {
       mbar_init(&sfull[s], 2);
       mbar_init(&sempty[s], 1);
     }
-    for (int b = 0; b < NB; ++b) {
+    for (int b = 0; b < NB * C::kHalves; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * C::kEpiWarps);
+      mbar_init(&tempty[b], 2 * C::kEpiWarps / C::kHalves);
     }
-    mbar_init(final_bar, 1);
+    mbar_init(final_bar, C::kHalves);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -952,7 +967,7 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
     for (int i = first; ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
       const int x_row = tile.t * 256 + int(rank) * kLanes;
-      const int w_row = tile.n * C::kBN + int(rank) * (C::kBN / 2);
+      const int w_row = tile.n * C::kBN + int(rank) * C::kBox;
       for (int kb = 0; kb < kbs; ++kb) {
         if (turn == mine) {
           ok = all_ok(mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, limit));
@@ -961,7 +976,10 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
             const uint32_t bar = bars + 8u * uint32_t(stage);
             tma_load_pair(sA + stage * kABytes, &tmX, kb * kKB, x_row, bar);
-            tma_load_pair(sB + stage * C::kBBytes, &tmW, kb * kKB, w_row, bar);
+#pragma unroll
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_pair(sB + stage * C::kBBytes + h * C::kBox * kKB, &tmW, kb * kKB,
+                            w_row + h * C::kN, bar);
           }
           __syncwarp();
         }
@@ -976,20 +994,23 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
     // the even CTA's barriers count both CTAs' bytes; the odd CTA stays until
     // the cluster barrier below
     if (rank == 0) filled.drain(full, STAGES, limit);
-  } else if (warp == 1 && rank == 0) {
-    // ---------------- MMA issuer, for both CTAs ----------------
+  } else if (warp >= 1 && warp <= C::kHalves && rank == 0) {
+    // ---------------- MMA issuers, for both CTAs ----------------
     // The whole warp walks the loop and one lane issues: operands computed by
     // a converged warp stay in uniform registers, where the MMA takes them.
     const bool leader = elect_one();
+    const int half = warp - 1;
     const uint64_t desc_a = make_sw128_desc(smem_u32(sA));
-    const uint64_t desc_b = make_sw128_desc(smem_u32(sB));
+    const uint64_t desc_b = make_sw128_desc(smem_u32(sB + half * C::kBox * kKB));
+    uint64_t* const my_tfull = tfull + half * NB;
+    uint64_t* const my_tempty = tempty + half * NB;
     int stage = 0, buf = 0, slot = 0;
     [[maybe_unused]] uint32_t sf = 0;  // TMEM of the quad's scales
     uint32_t phase = 0, bphase = 0, sphase = 0;
     bool ok = true;
     for (int i = first; ok && i < tiles; i += step) {
       if constexpr (MX) {
-        if (!all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit))) break;
+        if (!all_ok(mbar_wait_bounded(&my_tempty[buf], bphase ^ 1u, abort_flag, limit))) break;
         tc_fence_after();
       }
       for (int kb = 0; kb < kbs; ++kb) {
@@ -1010,14 +1031,16 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
             }
             __syncwarp();
           }
-        } else {
-          ok = all_ok(mbar_wait_bounded(&tempty[buf], bphase ^ 1u, abort_flag, limit));
-          if (!ok) break;
         }
         ok = all_ok(mbar_wait_bounded(&full[stage], phase, abort_flag, limit));
         if (!ok) break;
+        if constexpr (!MX) {
+          // last, since it is what the MMAs wait for
+          ok = all_ok(mbar_wait_bounded(&my_tempty[buf], bphase ^ 1u, abort_flag, limit));
+          if (!ok) break;
+        }
         tc_fence_after();
-        const uint32_t d = tmem_base + uint32_t(buf * C::kBN);
+        const uint32_t d = tmem_base + uint32_t(buf * C::kBN + half * C::kN);
         // descriptors of the stage's tiles; 32 bytes further along K are 2 units
         const uint64_t a0 = desc_a + uint32_t(stage * (kABytes / 16));
         const uint64_t b0 = desc_b + uint32_t(stage * (C::kBBytes / 16));
@@ -1040,13 +1063,13 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
             }
           }
         } else {
-          constexpr uint32_t idesc = make_idesc(1u, 0u, 256, C::kBN);
+          constexpr uint32_t idesc = make_idesc(1u, 0u, 256, C::kN);
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               tc_mma_f8_pair(d, a0 + 2 * kk, b0 + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+            tc_commit_pair(&my_tfull[buf]);
             tc_commit_pair(&empty[stage]);
-            tc_commit_pair(&tfull[buf]);
           }
           __syncwarp();
           if (++buf == NB) {
@@ -1061,7 +1084,7 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
       }
       if (!ok) break;
       if constexpr (MX) {
-        if (leader) tc_commit_pair(&tfull[buf]);
+        if (leader) tc_commit_pair(&my_tfull[buf]);
         __syncwarp();
         if (++buf == NB) {
           buf = 0;
@@ -1079,7 +1102,7 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
   } else if (MX && warp == 2) {
     // ---------------- scales: this CTA's tokens, all of the tile's weights ----------------
     const uint8_t* xs = static_cast<const uint8_t*>(p.xs);
-    const bool words = p.xs_blk == 1 && p.xs_row % 4 == 0 &&
+    const bool words = kbs >= 4 && p.xs_blk == 1 && p.xs_row % 4 == 0 &&
                        (reinterpret_cast<uintptr_t>(xs) & 3) == 0;
     const int64_t w_blocks = (p.N + 127) / 128;
     const int quads = (kbs + 3) / 4;
@@ -1129,7 +1152,9 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
     const int row = (warp & 3) * 32 + lane;
     const int col0 = ((warp - 4) >> 2) * COLS;
     const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(col0);
-    const uint32_t tempty0 = peer_addr(smem_u32(&tempty[0]), 0);
+    uint64_t* const my_tfull = tfull + (C::kHalves == 1 ? 0 : col0 / C::kN) * NB;
+    const uint32_t my_tempty =
+        peer_addr(smem_u32(tempty + (C::kHalves == 1 ? 0 : col0 / C::kN) * NB), 0);
     const int64_t w_blocks = (p.N + 127) / 128;
     constexpr int kVec = 16 / int(sizeof(TOUT));
     int buf = 0;
@@ -1141,7 +1166,7 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
       const int64_t n0 = int64_t(tile.n) * C::kBN + col0;
       float acc[COLS];
       if constexpr (MX) {
-        ok = mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit);
+        ok = mbar_wait_bounded(&my_tfull[buf], bphase, abort_flag, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -1155,7 +1180,7 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
         // the tile is in registers: the next one's MMAs may start
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_read(tempty0 + 8 * buf);
+        if (lane == 0) mbar_arrive_cluster_read(my_tempty + 8 * buf);
         if (++buf == NB) {
           buf = 0;
           bphase ^= 1u;
@@ -1167,33 +1192,42 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
         // the next k-block's scales are on their way while this one is added
-        float sx_n = __ldg(sx), sw_n = __ldg(sw);
+        float s = __ldg(sx) * __ldg(sw);
         for (int kb = 0; kb < kbs; ++kb) {
-          float s = sx_n * sw_n;
-          if (kb + 1 < kbs) {
-            sx_n = __ldg(sx + (kb + 1) * p.xs_blk);
-            sw_n = __ldg(sw + kb + 1);
-          }
-          ok = mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = all_ok(mbar_wait_bounded(&my_tfull[buf], bphase, abort_flag, limit));
           if (!ok) break;
           tc_fence_after();
           const uint32_t base = lane_base + uint32_t(buf * C::kBN);
+          // four batches of 32 columns, the third and fourth on their way while
+          // the first two are added
+          uint32_t v[2][32];
+          tmem_ld32(base, v[0]);
+          tmem_ld32(base + 32, v[1]);
+          tmem_ld_wait();
+          asm volatile("" : "+f"(s));  // no product can move before the wait
 #pragma unroll
-          for (int c = 0; c < COLS; c += BATCH) {
-            uint32_t v[BATCH];
-            tmem_ld32(base + c, v);
-            tmem_ld_wait();
-            asm volatile("" : "+f"(s));  // no product can move before the wait
-            if (c + BATCH >= COLS) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_read(tempty0 + 8 * buf);
-            }
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j)
-              acc[c + j] = fmaf(s, __uint_as_float(v[j]), acc[c + j]);
+            for (int j = 0; j < 32; ++j)
+              acc[32 * c + j] = fmaf(s, __uint_as_float(v[c][j]), acc[32 * c + j]);
+            tmem_ld32(base + 64 + 32 * c, v[c]);
           }
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_read(my_tempty + 8 * buf);
+          float s2 = s;
+          asm volatile("" : "+f"(s2));
+          if (kb + 1 < kbs) {
+            sx += p.xs_blk;
+            ++sw;
+            s = __ldg(sx) * __ldg(sw);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              acc[64 + 32 * c + j] = fmaf(s2, __uint_as_float(v[c][j]), acc[64 + 32 * c + j]);
           if (++buf == NB) {
             buf = 0;
             bphase ^= 1u;
@@ -1450,8 +1484,9 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   st = encode_tma_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, uint64_t(inner),
                      uint64_t(num_rows), uint64_t(ld_x), kKB, x_box);
   if (st != MOE_OK) return st;
+  const uint32_t w_box = plan.pair ? (mx ? PairCfg<true>::kBox : PairCfg<false>::kBox) : kLanes;
   st = encode_tma_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, uint64_t(inner),
-                     uint64_t(out_cols), uint64_t(ld_w), kKB, kLanes);
+                     uint64_t(out_cols), uint64_t(ld_w), kKB, w_box);
   if (st != MOE_OK) return st;
   MatmulParams p = {};
   p.xs = x_scale;
