@@ -566,32 +566,53 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
         }
       }
     } else {
-      for (int i = first; ok && i < tiles; i += step) {
+      // sx * sw of four k-blocks at a time, loaded together and a turn ahead
+      constexpr int R = (BN + 31) / 32, U = 4;
+      const float* xs = static_cast<const float*>(p.xs);
+      float v[U][R];
+      auto fetch = [&](int i, int k0) {
         const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
-        const float* xs = static_cast<const float*>(p.xs);
         const float* ws = static_cast<const float*>(p.ws) + int64_t(tile.n) * p.kb_total;
-        constexpr int R = (BN + 31) / 32;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const float w = __ldg(ws + kb);
-          float v[R];
+        const float* at[R];
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const int64_t t = int64_t(tile.t) * BN + 32 * r + lane;
-            v[r] = t < p.T && 32 * r + lane < BN ? __ldg(xs + t * p.xs_row + kb * p.xs_blk) : 0.0f;
-          }
-          ok = mbar_wait_bounded(&sempty[slot], sphase ^ 1u, abort_flag, limit);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          float* dst = reinterpret_cast<float*>(sRing) + slot * BN;
+        for (int r = 0; r < R; ++r)  // tokens past the last one repeat it
+          at[r] = xs + min(int64_t(tile.t) * BN + 32 * r + lane, p.T - 1) * p.xs_row;
+        float w[U];
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (32 * r + lane < BN) dst[32 * r + lane] = v[r] * w;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sfull[slot]);
-          if (++slot == SLOTS) {
-            slot = 0;
-            sphase ^= 1u;
+        for (int u = 0; u < U; ++u) {
+          const int kb = min(k0 + u, kb1 - 1);
+          w[u] = __ldg(ws + kb);
+#pragma unroll
+          for (int r = 0; r < R; ++r) v[u][r] = __ldg(at[r] + kb * p.xs_blk);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) v[u][r] *= w[u];
+      };
+      if (first < tiles) fetch(first, kb0);
+      for (int i = first; ok && i < tiles; i += step) {
+        for (int k0 = kb0; ok && k0 < kb1; k0 += U) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (k0 + u >= kb1) break;
+            ok = all_ok(mbar_wait_bounded(&sempty[slot], sphase ^ 1u, abort_flag, limit));
+            if (!ok) break;
+            float* dst = reinterpret_cast<float*>(sRing) + slot * BN;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+              if (32 * r + lane < BN) dst[32 * r + lane] = v[u][r];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sfull[slot]);
+            if (++slot == SLOTS) {
+              slot = 0;
+              sphase ^= 1u;
+            }
           }
+          if (k0 + U < kb1)
+            fetch(i, k0 + U);
+          else if (i + step < tiles)
+            fetch(i + step, kb0);
         }
       }
     }
