@@ -548,6 +548,23 @@ int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale, int64_t xs_
                    const void* addend, int64_t ld_addend, void* out, int64_t ld_out,
                    int out_dtype, int32_t* status, void* stream);
 
+/*
+ * The SwiGLU MLP of a shared expert: out = w2 (silu(g) * u) (+ addend), [g | u]
+ * = w13 x. x, addend and out [num_rows, hidden] in dtype (F32/F16/BF16), w13
+ * [2 * inter, hidden] (gate rows, then up rows) and w2 [hidden, inter] e4m3 with
+ * dense block scales in scale_format, in which the activations are quantised
+ * per row and 128 columns; [g | u] is held in dtype. addend may be NULL or out.
+ * Four launches: moe_fp8_quantize_rows, moe_fp8_matmul, the gated quantiser,
+ * moe_fp8_matmul. Calls that may overlap need workspaces of their own.
+ */
+int moe_fp8_swiglu_mlp_workspace_size(int64_t num_rows, int64_t hidden, int64_t inter, int dtype,
+                                      int scale_format, size_t* bytes);
+int moe_fp8_swiglu_mlp(const void* x, int64_t ld_x, int dtype, int64_t num_rows, int64_t hidden,
+                       int64_t inter, const void* w13, int64_t ld_w13, const void* w13_scale,
+                       const void* w2, int64_t ld_w2, const void* w2_scale, int scale_format,
+                       const void* addend, int64_t ld_addend, void* out, int64_t ld_out,
+                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 /* How moe_fp8_matmul runs these sizes with 16-byte aligned 16-bit output rows
  * (no GPU needed, for 148 SMs): info[0] 1 when pairs of CTAs share tiles of 256
  * tokens on the MMA's rows (0: the weights lie there), [1] columns per tile,

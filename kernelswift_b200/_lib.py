@@ -111,6 +111,10 @@ SIGNATURES = {
     "moe_fp8_quantize_blocks": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp]),
     "moe_fp8_matmul": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64,
                               _vp, _i64, _vp, _i64, _int, _vp, _vp]),
+    "moe_fp8_swiglu_mlp_workspace_size": (_int, [_i64, _i64, _i64, _int, _int,
+                                                 ctypes.POINTER(_sz)]),
+    "moe_fp8_swiglu_mlp": (_int, [_vp, _i64, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64,
+                                  _vp, _int, _vp, _i64, _vp, _i64, _vp, _sz, _vp, _vp]),
     "moe_fp8_matmul_plan": (_int, [_i64, _i64, _i64, _int, _vp]),
     "moe_combine_rows": (_int, [_vp, _int, _vp, _vp, _int, _i64, _int, _i64, _vp, _int, _vp]),
     "moe_selftest_wait_timeout": (_int, [_vp, _int, _vp]),

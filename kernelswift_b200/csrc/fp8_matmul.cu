@@ -48,6 +48,7 @@ struct MatmulParams {
   int kb_total;            // k-blocks
   int t_tiles, n_tiles;
   int splits;              // CTAs of a cluster that share a tile
+  int slice;               // tokens that each of them sums (kPush): a multiple of 4
   int32_t* status;
   uint64_t wait_limit_ns;
 };
@@ -69,6 +70,21 @@ __device__ __forceinline__ Tile tile_at(int i, int t_tiles, int n_tiles) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address `addr` of this CTA in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+// Stores 16 bytes into a CTA of the cluster; they are counted on its barrier.
+__device__ __forceinline__ void st_async4(uint32_t addr, const float* v, uint32_t bar) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, "
+      "[%5];" ::"r"(addr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+      "r"(__float_as_uint(v[3])), "r"(bar)
+      : "memory");
 }
 // Shared-memory word of CTA `rank` at this CTA's address `addr`.
 __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
@@ -139,6 +155,15 @@ struct Filled {
       }
   }
 };
+
+// Asks L2 to fetch the box at (c0, c1); nothing reaches the SM, nothing waits.
+__device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* tm, int32_t c0, int32_t c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(tm)),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
+constexpr int kL2Ahead = 6;   // k-blocks of weights a CTA asks for ahead of the wait
 
 // TMA producers: two warps take the stages in turn. A turn (wait for the
 // stage, announce its bytes, issue two copies) takes a warp about 490 cycles
@@ -237,7 +262,14 @@ struct ColsCfg {
   static constexpr int kRingBytes =
       MX ? kSfSlots * kQuads * kQuadBytes : kFacSlots * BN * 4;
   static constexpr int kGroups = kEpiWarps / 4;       // epilogue groups of 128 lanes
-  static constexpr size_t kFixed = 1024 + 512 + kRingBytes + size_t(kGroups) * 2 * kStagedBytes;
+  // A split tile's partials: pushed into the memory of the CTA that sums them
+  // where that costs no pipeline stages (BN <= 32), else read from their own
+  // CTA's memory.
+  static constexpr bool kPush = BN <= 32;
+  static constexpr int kRecvBytes = kPush ? 16384 : 0;
+  static constexpr int kOutBytes =  // staged output, or received partials
+      kGroups * 2 * kStagedBytes > kRecvBytes ? kGroups * 2 * kStagedBytes : kRecvBytes;
+  static constexpr size_t kFixed = 1024 + 512 + kRingBytes + size_t(kOutBytes);
   static constexpr int kStages = int(((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / kStageBytes);
   static constexpr size_t kSmem = kFixed + size_t(kStages) * kStageBytes;
   // TMEM: accumulators (UE8M0) or per-k-block buffers (fp32), then scale slots
@@ -249,7 +281,7 @@ struct ColsCfg {
   static_assert(kUsed <= 512 && kTmem * kCtas <= 512, "TMEM columns");
   static_assert(size_t(kStages) * kStageBytes >= size_t(BN) * kLanes * 4,
                 "the partial tile reuses the stages");
-  static_assert(8 * (2 * kStages + 2 * kFacSlots + 2 * 4 + 1) + 8 <= 512, "barriers");
+  static_assert(8 * (2 * kStages + 2 * kFacSlots + 2 * 4 + 2) + 8 <= 512, "barriers");
 };
 
 template <bool MX, int BN, typename TOUT>
@@ -269,19 +301,21 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   uint8_t* sB = sA + STAGES * kABytes;
   uint8_t* sRing = sB + STAGES * C::kBBytes;
   uint8_t* sOut = sRing + C::kRingBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + C::kGroups * 2 * kStagedBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + C::kOutBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* sfull = empty + STAGES;
   uint64_t* sempty = sfull + SLOTS;
   uint64_t* tfull = sempty + SLOTS;
   uint64_t* tempty = tfull + NB;
   uint64_t* final_bar = tempty + NB;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+  uint64_t* recv_bar = final_bar + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(recv_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   // the warp's number, known to be the same for all its lanes
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
+  const bool push = C::kPush && p.splits > 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -296,8 +330,11 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
       mbar_init(&tempty[b], C::kEpiWarps);
     }
     mbar_init(final_bar, 1);
+    mbar_init(recv_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tmW);  // kernel arguments, no predecessor's data
+    tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmem);
@@ -307,8 +344,10 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  pdl_wait();
-  pdl_trigger();
+  if (push) {
+    __syncwarp();
+    cluster_sync();  // every CTA's recv_bar is ready
+  }
 
   const uint64_t limit = p.wait_limit_ns;
   const int tiles = p.t_tiles * p.n_tiles;
@@ -317,6 +356,16 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   const int first = int(blockIdx.x) / p.splits, step = int(gridDim.x) / p.splits;
   const int kb0 = int(int64_t(p.kb_total) * part / p.splits);
   const int kb1 = int(int64_t(p.kb_total) * (part + 1) / p.splits);
+  // While the previous kernel finishes, the weights of this CTA's first tile
+  // start on their way to L2. Should that kernel be writing them, no harm is
+  // done: nothing is read before the wait, and L2 is where its writes land.
+  if (warp == 0 && first < tiles && elect_one()) {
+    const int row = tile_at(first, p.t_tiles, p.n_tiles).n * kLanes;
+    for (int kb = kb0; kb < min(kb1, kb0 + kL2Ahead); ++kb) l2_prefetch_2d(&tmW, kb * kKB, row);
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
 
   float acc[COLS];  // the epilogue warps' tile columns
 #pragma unroll
@@ -389,10 +438,6 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   if (producer_of(warp) >= 0) {
     // ---------------- TMA producers ----------------
     const bool leader = elect_one();
-    if (leader) {
-      tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmX);
-    }
     const int mine = producer_of(warp);
     int stage = 0, turn = 0;
     uint32_t phase = 0;
@@ -625,6 +670,11 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     int buf = 0, slot = 0;
     uint32_t bphase = 0, sphase = 0;
     constexpr int BATCH = COLS >= 32 ? 32 : 16;
+    if (push && threadIdx.x == 128) {
+      const int64_t t0 = int64_t(tile_at(first, p.t_tiles, p.n_tiles).t) * BN + part * p.slice;
+      if (part * p.slice < BN && t0 < p.T)
+        mbar_arrive_expect_tx(recv_bar, uint32_t(p.splits * p.slice * kLanes * 4));
+    }
     for (int i = first; epi_ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
       if constexpr (MX) {
@@ -702,6 +752,20 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
       }
       if (p.splits == 1) {
         store_tile(tile, col0, row, group);
+      } else if constexpr (C::kPush) {
+        // tokens [o * ts, (o + 1) * ts) go to CTA o of the cluster, as
+        // [source][weight row][token]
+        const int ts = p.slice;
+        const int live = int(min(int64_t(BN), p.T - int64_t(tile.t) * BN));
+        const uint32_t dst = smem_u32(sOut) + 4u * uint32_t((part * kLanes + row) * ts);
+        const uint32_t bar = smem_u32(recv_bar);
+#pragma unroll
+        for (int j = 0; j < COLS; j += 4) {
+          const int o = j / ts;
+          if (o * ts < live)
+            st_async4(peer_addr(dst + 4u * uint32_t(j - o * ts), uint32_t(o)), &acc[j],
+                      peer_addr(bar, uint32_t(o)));
+        }
       } else {
         // every MMA of this CTA's only tile has completed, so the stages are
         // free; [token][weight row], a warp writes 32 neighbouring words
@@ -713,8 +777,42 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
   }
 
   __syncwarp();
+  if (push) {
+    // a CTA leaves once all have arrived here, their stores to it on the way
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    const Tile tile = tile_at(first, p.t_tiles, p.n_tiles);
+    const int64_t n = int64_t(tile.n) * kLanes + (threadIdx.x & 127);
+    const int ts = p.slice, j0 = part * ts;
+    const int64_t t0 = int64_t(tile.t) * BN + j0;
+    if (warp >= 4 && j0 < BN && t0 < p.T) {
+      bool ok = mbar_wait_bounded(recv_bar, 0, abort_flag, limit);
+      if (all_ok(ok) && !*abort_flag && n < p.N) {
+        const float4* src = reinterpret_cast<const float4*>(sOut) + (threadIdx.x & 127) * (ts / 4);
+        for (int j = 0; j < ts; j += 4) {
+          float4 sum = src[j / 4];
+          for (int r = 1; r < p.splits; ++r) {  // in rank order
+            const float4 v = src[r * kLanes * (ts / 4) + j / 4];
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+          }
+          const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t t = t0 + j + e;
+            if (j0 + j + e < BN && t < p.T) {
+              float v = out[e];
+              if (p.add != nullptr)
+                v += to_f32(static_cast<const TOUT*>(p.add)[t * p.ld_add + n]);
+              static_cast<TOUT*>(p.out)[t * p.ld_out + n] = from_f32<TOUT>(v);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   __syncthreads();
-  if (p.splits > 1) {
+  if (p.splits > 1 && !push) {
     cluster_sync();
     // CTA r sums tokens r, r + splits, ... over the cluster, in rank order
     const Tile tile = tile_at(first, p.t_tiles, p.n_tiles);
@@ -793,12 +891,6 @@ struct PairCfg {
                 "setmaxnreg split");
 };
 
-// Shared-memory address `addr` of this CTA in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
-}
 // Arrives on a barrier of the cluster, after this thread's (and, after a warp
 // barrier, its warp's) writes.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
@@ -1325,6 +1417,8 @@ Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, bool vec, int sms) {
     if (bn > 16 && bn / 2 >= T) continue;  // the half would hold every token
     const int64_t tiles = ceil_div(T, bn) * ceil_div(N, kLanes);
     for (int s = 1; s <= 8 && s <= kbs; ++s) {
+      // the partials that a CTA receives fit their buffer for powers of two
+      if (bn == 32 && (s & (s - 1)) != 0) continue;
       const int occ = bn <= 64 ? 2 : 1;
       if (s > 1 && tiles * s > int64_t(sms) * occ) break;
       // cycles: k-blocks one after another on an SM, each the MMA's or, when
@@ -1524,6 +1618,7 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   p.t_tiles = int(ceil_div(num_rows, plan.pair ? 256 : plan.bn));
   p.n_tiles = int(ceil_div(out_cols, plan.pair ? plan.bn : kLanes));
   p.splits = plan.splits;
+  p.slice = int(round_up(ceil_div(plan.bn, plan.splits), 4));
   p.status = status;
   p.wait_limit_ns = kWaitLimitNs;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -14,6 +14,9 @@ CUDA graph. There is no CPU path and no gradient: these are serving operators.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -59,6 +62,28 @@ def _fp8_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     q = _empty_fp8(rows, cols, t.device)
     q.view(torch.uint8).copy_(t.view(torch.uint8))
     return q
+
+
+def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, index: int) -> None:
+    if (out.shape != (rows, cols) or out.get_device() != index or out.dtype != dtype
+            or dtype not in _FLOAT or out.stride(1) != 1 and cols > 1
+            or out.stride(0) < cols and rows > 1):
+        raise ValueError(f"out must be a bf16, f16 or f32 [{rows}, {cols}] tensor with dense rows "
+                         "on the operands' device")
+    _no_grad_needed("out", out)
+
+
+def _addend(addend: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype, index: int):
+    """(pointer, row stride) of the addend, (None, 0) without one."""
+    if addend is None:
+        return None, 0
+    _no_grad_needed("addend", addend)
+    if addend.shape != (rows, cols) or addend.dtype != dtype or addend.get_device() != index:
+        raise ValueError(f"addend must be a {dtype} [{rows}, {cols}] tensor on the operands' "
+                         "device")
+    if addend.numel() and (addend.stride(1) != 1 or addend.stride(0) < cols and rows > 1):
+        raise ValueError("addend must have dense rows")
+    return addend.data_ptr(), max(addend.stride(0), cols)
 
 
 def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = False
@@ -152,24 +177,14 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         out = torch.empty(T, N, dtype=out_dtype, device=x.device)
     else:
         out_dtype = out.dtype
-        if (out.shape != (T, N) or out.get_device() != index or out_dtype not in _FLOAT
-                or out.stride(1) != 1 and N > 1 or out.stride(0) < N and T > 1):
-            raise ValueError(f"out must be a bf16, f16 or f32 [{T}, {N}] tensor with dense rows "
-                             f"on {x.device}")
-        _no_grad_needed("out", out)
-    add_ptr = add_ld = 0
-    if addend is not None:
-        _no_grad_needed("addend", addend)
-        if addend.shape != (T, N) or addend.dtype != out_dtype or addend.get_device() != index:
-            raise ValueError(f"addend must be a {out_dtype} [{T}, {N}] tensor on {x.device}")
-        addend = _rows_of(addend)
-        add_ptr, add_ld = addend.data_ptr(), max(addend.stride(0), N)
+        _check_out(out, T, N, out_dtype, index)
+    add_ptr, add_ld = _addend(addend, T, N, out_dtype, index)
     if not w_scale.is_contiguous():
         w_scale = w_scale.contiguous()
     pitch = _round_up(K, 16)
     _enqueue("moe_fp8_matmul", index, x.data_ptr(), max(x.stride(0), pitch), x_scale.data_ptr(),
              x_scale.stride(0), x_scale.stride(1), w.data_ptr(), max(w.stride(0), pitch),
-             w_scale.data_ptr(), fmt, T, N, K, add_ptr or None, add_ld, out.data_ptr(),
+             w_scale.data_ptr(), fmt, T, N, K, add_ptr, add_ld, out.data_ptr(),
              max(out.stride(0), N), _DTYPE_CODE[out_dtype],
              None if status is None else status.data_ptr())
     return out
@@ -178,27 +193,64 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
 def block_matmul_plan(num_rows: int, out_cols: int, inner: int, scale_format: str = "ue8m0"
                       ) -> dict:
     """How block_matmul runs these sizes (moe_fp8_matmul_plan; no GPU needed)."""
-    import ctypes
-
     info = (ctypes.c_int32 * 4)()
     _lib.call("moe_fp8_matmul_plan", num_rows, out_cols, inner, _FORMAT[scale_format], info)
     return dict(zip(("cta_pairs", "tile_cols", "splits", "ctas"), list(info)))
 
 
+@functools.lru_cache(maxsize=256)
+def _mlp_workspace_bytes(T: int, H: int, inter: int, dtype: int, fmt: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.call("moe_fp8_swiglu_mlp_workspace_size", T, H, inter, dtype, fmt, ctypes.byref(n))
+    return n.value
+
+
 def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
                w2_scale: torch.Tensor, addend: torch.Tensor | None = None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
-    """The SwiGLU MLP of a shared expert on block-scaled e4m3 weights:
-    w2 (silu(w1 x) * (w3 x)) (+ addend), x [T, H] (f32/f16/bf16), w13 [2I, H]
-    (gate rows, then up rows), w2 [H, I]. Activations are quantised per token
-    and 128 columns in the weights' scale format; the gate-up product is held
-    in x's dtype. addend [T, H] in x's dtype (the routed experts' output) is
-    added before the one rounding of the result. Four launches."""
-    if w13.dim() != 2 or w2.dim() != 2 or w13.shape[0] != 2 * w2.shape[1]:
-        raise ValueError(f"w13 {tuple(w13.shape)} must be [2I, H] for w2 {tuple(w2.shape)}")
-    if w13_scale.dtype not in _SCALE_FORMAT:
-        raise ValueError("w13_scale must be float32 or uint8 (UE8M0)")
-    fmt = "fp32" if w13_scale.dtype == torch.float32 else "ue8m0"
-    both = block_matmul(*quantize_rows(x, fmt), w13, w13_scale, out_dtype=x.dtype)
-    return block_matmul(*quantize_rows(both, fmt, gated=True), w2, w2_scale, out_dtype=x.dtype,
-                        addend=addend, out=out)
+               out: torch.Tensor | None = None, status: torch.Tensor | None = None
+               ) -> torch.Tensor:
+    """The SwiGLU MLP of a shared expert on block-scaled e4m3 weights
+    (moe_fp8_swiglu_mlp): w2 (silu(g) * u) (+ addend), [g | u] = w13 x, for
+    x [T, H] (f32/f16/bf16), w13 [2I, H] (gate rows, then up rows) and w2 [H, I]
+    with their scales, all float32 or all uint8 (UE8M0). Activations are
+    quantised per token and 128 columns in the weights' scale format; [g | u] is
+    held in x's dtype. addend [T, H] in x's dtype (the routed experts' output; it
+    may be out) is added before the one rounding of the result. Four launches."""
+    index = x.get_device()
+    for name, t in (("x", x), ("w13", w13), ("w13_scale", w13_scale), ("w2", w2),
+                    ("w2_scale", w2_scale)):
+        if t.get_device() != index or index < 0:
+            _check_cuda(name, t)
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    _no_grad_needed("x", x)
+    if x.dim() != 2 or x.dtype not in _FLOAT or x.shape[1] < 1:
+        raise ValueError("x must be a 2-D f32/f16/bf16 tensor")
+    w13, w2 = _fp8_rows("w13", w13), _fp8_rows("w2", w2)
+    (T, H), inter = x.shape, w2.shape[1]
+    if w13.shape != (2 * inter, H) or w2.shape[0] != H or inter < 1:
+        raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} must be [2I, {H}] and "
+                         f"[{H}, I]")
+    fmt = _SCALE_FORMAT.get(w13_scale.dtype)
+    if fmt is None or w2_scale.dtype != w13_scale.dtype:
+        raise ValueError("w13_scale and w2_scale must both be float32 or both uint8 (UE8M0)")
+    hb, ib = -(-H // 128), -(-inter // 128)
+    if w13_scale.shape != (-(-2 * inter // 128), hb) or w2_scale.shape != (hb, ib):
+        raise ValueError(f"scales must be [{-(-2 * inter // 128)}, {hb}] and [{hb}, {ib}], got "
+                         f"{tuple(w13_scale.shape)} and {tuple(w2_scale.shape)}")
+    x = _rows_of(x)
+    if out is None:
+        out = torch.empty(T, H, dtype=x.dtype, device=x.device)
+    else:
+        _check_out(out, T, H, x.dtype, index)
+    add_ptr, add_ld = _addend(addend, T, H, x.dtype, index)
+    code = _DTYPE_CODE[x.dtype]
+    # of its own: a workspace kept by stream would be shared by captured graphs
+    ws = torch.empty(_mlp_workspace_bytes(T, H, inter, code, fmt), dtype=torch.uint8,
+                     device=x.device)
+    w13_scale, w2_scale = w13_scale.contiguous(), w2_scale.contiguous()
+    _enqueue("moe_fp8_swiglu_mlp", index, x.data_ptr(), max(x.stride(0), H), code, T, H, inter,
+             w13.data_ptr(), max(w13.stride(0), _round_up(H, 16)), w13_scale.data_ptr(),
+             w2.data_ptr(), max(w2.stride(0), _round_up(inter, 16)), w2_scale.data_ptr(), fmt,
+             add_ptr, add_ld, out.data_ptr(), max(out.stride(0), H), ws.data_ptr(), ws.numel(),
+             None if status is None else status.data_ptr())
+    return out
