@@ -9,14 +9,17 @@
 // down product's operand is written straight from the gate-up product.
 // Blocks: the same with one scale for each 128 x 128 block (weights).
 //
-// x * 448 / absmax is computed as (x * 0.875) / (absmax * 2^-9), one IEEE
-// division: for 16-bit inputs numerator and denominator are exact, so a
-// quotient on the midpoint of two e4m3 values is recognised as such (a
-// multiplication by a rounded reciprocal falls to either side of it).
+// x * 448 / absmax is the IEEE quotient (x * 0.875) / (absmax * 2^-9): for
+// 16-bit inputs numerator and denominator are exact, so a quotient on the
+// midpoint of two e4m3 values is recognised as such (a multiplication by a
+// rounded reciprocal falls to either side of it). Only those near a midpoint
+// are divided: the product with the reciprocal, off by less than 2^-22, decides
+// every quotient whose two bounds round to the same e4m3 value.
 //
 // What bounds the row kernel: HBM. A half-warp holds a group (8 columns per
-// lane, one 16-byte load for 16-bit inputs), a warp 1024 columns of a row with
-// its four loads in flight before the first is used.
+// lane, one 16-byte load for 16-bit inputs), a warp up to 1024 columns of a row
+// with its loads in flight before the first is used; neighbouring warps take
+// neighbouring columns, so that a block reads one run of memory.
 #include <type_traits>
 
 #include "common.cuh"
@@ -25,8 +28,6 @@ namespace ksw {
 namespace {
 
 constexpr int kRowWarps = 8;
-constexpr int kChunk = 1024;  // columns of a row per warp
-constexpr int kIters = kChunk / 256;
 
 struct QuantRows {
   const void* x;
@@ -81,86 +82,94 @@ __device__ __forceinline__ float fp32_scale(float amax) {
   return amax > 0.0f ? amax / 448.0f : 1.0f;
 }
 
-template <typename Tin, bool VEC, bool GATED, bool UE8M0>
+// Two values over den, rounded to e4m3: by the reciprocal where both its bounds
+// agree, else divided.
+__device__ __forceinline__ uint32_t e4m3x2_over(float a, float b, float den, float inv) {
+  constexpr float kLo = 1.0f - 0x1p-22f, kHi = 1.0f + 0x1p-22f;
+  const float x = a * inv, y = b * inv;
+  uint32_t q = e4m3x2(x * kLo, y * kLo);
+  if (q != e4m3x2(x * kHi, y * kHi)) q = e4m3x2(a / den, b / den);
+  return q;
+}
+
+// ITERS: runs of 256 columns per warp. One row's warps follow one another.
+template <typename Tin, bool VEC, bool GATED, bool UE8M0, int ITERS>
 __global__ void __launch_bounds__(32 * kRowWarps)
-    fp8_quantize_rows_kernel(const QuantRows p, int chunks) {
+    fp8_quantize_rows_kernel(const QuantRows p, uint32_t chunks) {
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the warps of a block take neighbouring rows at the same columns, so that
-  // their scales meet in the same sectors
-  const int64_t t = int64_t(blockIdx.x) * kRowWarps + warp;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+  const int64_t t = unit / chunks;
   if (t >= p.T) return;
-  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
-    const int64_t c0 = int64_t(chunk) * kChunk + 8 * lane;
-    const Tin* row = static_cast<const Tin*>(p.x) + t * p.ld_x;
-    float v[kIters][8];
-    float u[GATED ? kIters : 1][8];
+  const int64_t c0 = int64_t(uint32_t(unit - t * chunks)) * (256 * ITERS) + 8 * lane;
+  const Tin* row = static_cast<const Tin*>(p.x) + t * p.ld_x;
+  float v[ITERS][8];
+  float u[GATED ? ITERS : 1][8];
 #pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-      const int64_t c = c0 + 256 * i;
-      const int n = int(min(int64_t(8), max(int64_t(0), p.K - c)));
-      load8<Tin, VEC>(row + c, n, v[i]);
-      if constexpr (GATED) load8<Tin, VEC>(row + p.K + c, n, u[i]);
+  for (int i = 0; i < ITERS; ++i) {
+    const int64_t c = c0 + 256 * i;
+    const int n = int(min(int64_t(8), max(int64_t(0), p.K - c)));
+    load8<Tin, VEC>(row + c, n, v[i]);
+    if constexpr (GATED) load8<Tin, VEC>(row + p.K + c, n, u[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    const int64_t c = c0 + 256 * i;
+    float amax = 0.0f;
+    [[maybe_unused]] float gate[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (GATED) {
+        gate[e] = v[i][e];
+        v[i][e] = silu_up(v[i][e], u[i][e]);
+      }
+      amax = fmaxf(amax, fabsf(v[i][e]));
     }
 #pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-      const int64_t c = c0 + 256 * i;
-      float amax = 0.0f;
-      [[maybe_unused]] float gate[8];
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    uint32_t w[4];
+    const int64_t blk = c / 128;
+    const bool writer = (lane & 15) == 0 && c < p.K;
+    if constexpr (UE8M0) {
+      uint32_t b = ue8m0_byte(amax);
+      if constexpr (GATED) {
+        // a maximum within the rounding of the 32-bit silu (under 8 ulp) of
+        // 448 * 2^k decides the scale by its 64-bit value
+        const uint32_t bits = __float_as_uint(amax);
+        const int off = int(bits & 0x7fffffu) - 0x600000;
+        const bool near = amax > 0.0f && amax < INFINITY && off >= -16 && off <= 16;
+        if (__any_sync(0xffffffffu, near)) {
+          double m = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (GATED) {
-          gate[e] = v[i][e];
-          v[i][e] = silu_up(v[i][e], u[i][e]);
-        }
-        amax = fmaxf(amax, fabsf(v[i][e]));
-      }
+          for (int e = 0; e < 8; ++e)
+            m = fmax(m, fabs(silu_up(double(gate[e]), double(u[i][e]))));
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1)
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      uint32_t w[4];
-      const int64_t blk = c / 128;
-      const bool writer = (lane & 15) == 0 && c < p.K;
-      if constexpr (UE8M0) {
-        uint32_t b = ue8m0_byte(amax);
-        if constexpr (GATED) {
-          // a maximum within the rounding of the 32-bit silu (under 8 ulp) of
-          // 448 * 2^k decides the scale by its 64-bit value
-          const uint32_t bits = __float_as_uint(amax);
-          const int off = int(bits & 0x7fffffu) - 0x600000;
-          const bool near = amax > 0.0f && amax < INFINITY && off >= -16 && off <= 16;
-          if (__any_sync(0xffffffffu, near)) {
-            double m = 0.0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              m = fmax(m, fabs(silu_up(double(gate[e]), double(u[i][e]))));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (near) {
-              const int e = int(bits >> 23);
-              const double border = ldexp(1.75, e - 127);
-              b = uint32_t(min(max(e - 8 + (m > border ? 1 : 0), 0), 254));
-            }
+          for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (near) {
+            const int e = int(bits >> 23);
+            const double border = ldexp(1.75, e - 127);
+            b = uint32_t(min(max(e - 8 + (m > border ? 1 : 0), 0), 254));
           }
         }
-        const float inv = ue8m0_inv_scale(b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
-        if (writer) static_cast<uint8_t*>(p.scale)[t * p.s_row + blk * p.s_blk] = uint8_t(b);
-      } else {
-        const Ratio r = ratio_of(amax);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = e4m3x2(v[i][2 * e] * r.num / r.den, v[i][2 * e + 1] * r.num / r.den);
-        if (writer) static_cast<float*>(p.scale)[t * p.s_row + blk * p.s_blk] = fp32_scale(amax);
       }
-      // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
-      // 8 bytes at a column below K are inside the row
-      if (c < p.K)
-        *reinterpret_cast<uint2*>(p.q + t * p.ld_q + c) =
-            make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+      const float inv = ue8m0_inv_scale(b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
+      if (writer) static_cast<uint8_t*>(p.scale)[t * p.s_row + blk * p.s_blk] = uint8_t(b);
+    } else {
+      const Ratio r = ratio_of(amax);
+      const float inv = 1.0f / r.den;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = e4m3x2_over(v[i][2 * e] * r.num, v[i][2 * e + 1] * r.num, r.den, inv);
+      if (writer) static_cast<float*>(p.scale)[t * p.s_row + blk * p.s_blk] = fp32_scale(amax);
     }
+    // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
+    // 8 bytes at a column below K are inside the row
+    if (c < p.K)
+      *reinterpret_cast<uint2*>(p.q + t * p.ld_q + c) =
+          make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
   }
 }
 
@@ -213,18 +222,28 @@ __global__ void __launch_bounds__(32 * kBlkWarps)
     }
 }
 
+template <typename Tin, bool VEC, bool GATED, int ITERS>
+int launch_rows_i(const QuantRows& p, int ue8m0, cudaStream_t s) {
+  const int64_t chunks = ceil_div(p.K, 256 * ITERS);
+  const int64_t blocks = ceil_div(p.T * chunks, kRowWarps);
+  KSW_REQUIRE(blocks < (int64_t(1) << 31), MOE_ERR_UNSUPPORTED,
+              "fp8_quantize_rows: too many blocks");
+  if (ue8m0)
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, true, ITERS>, dim3(unsigned(blocks)),
+               dim3(32 * kRowWarps), 0, s, p, uint32_t(chunks));
+  else
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, false, ITERS>, dim3(unsigned(blocks)),
+               dim3(32 * kRowWarps), 0, s, p, uint32_t(chunks));
+  return MOE_OK;
+}
+
 template <typename Tin, bool VEC, bool GATED>
 int launch_rows(const QuantRows& p, int ue8m0, cudaStream_t s) {
-  const int64_t row_blocks = ceil_div(p.T, kRowWarps);
-  const int chunks = int(ceil_div(p.K, kChunk));
-  const dim3 grid(unsigned(row_blocks), unsigned(std::min(chunks, 65535)));
-  if (ue8m0)
-    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, true>, grid, dim3(32 * kRowWarps), 0, s,
-               p, chunks);
-  else
-    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, false>, grid, dim3(32 * kRowWarps), 0, s,
-               p, chunks);
-  return MOE_OK;
+  // 256 columns per warp until the SMs are full of warps, then more loads in
+  // flight per warp
+  constexpr int kMany = GATED || sizeof(Tin) == 4 ? 2 : 4;
+  if (p.T * ceil_div(p.K, 256) <= 148 * 64) return launch_rows_i<Tin, VEC, GATED, 1>(p, ue8m0, s);
+  return launch_rows_i<Tin, VEC, GATED, kMany>(p, ue8m0, s);
 }
 
 template <typename Tin>
