@@ -12,14 +12,13 @@
 // x * 448 / absmax is the IEEE quotient (x * 0.875) / (absmax * 2^-9): for
 // 16-bit inputs numerator and denominator are exact, so a quotient on the
 // midpoint of two e4m3 values is recognised as such (a multiplication by a
-// rounded reciprocal falls to either side of it). Only those near a midpoint
-// are divided: the product with the reciprocal, off by less than 2^-22, decides
-// every quotient whose two bounds round to the same e4m3 value.
+// rounded reciprocal falls to either side of it).
 //
 // What bounds the row kernel: HBM. A half-warp holds a group (8 columns per
-// lane, one 16-byte load for 16-bit inputs), a warp up to 1024 columns of a row
-// with its loads in flight before the first is used; neighbouring warps take
-// neighbouring columns, so that a block reads one run of memory.
+// lane, one 16-byte load for 16-bit inputs, two where rows start off such a
+// boundary), a warp up to 1024 columns of a row with its loads in flight before
+// the first is used; neighbouring warps take neighbouring columns, so that a
+// block reads one run of memory.
 #include <type_traits>
 
 #include "common.cuh"
@@ -38,25 +37,53 @@ struct QuantRows {
   int64_t s_row, s_blk;  // strides of the scale, in elements
 };
 
-// Eight consecutive elements from `p`, of which `n` exist (the rest are 0).
-template <typename Tin, bool VEC>
-__device__ __forceinline__ void load8(const Tin* p, int n, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (n >= 8) {
-      if constexpr (std::is_same<Tin, float>::value) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const Tin* e = reinterpret_cast<const Tin*>(&a);
+// Eight consecutive elements, as the aligned 16-byte vectors that hold them
+// (each holds at least one of their bytes) and, unless all rows start on such
+// boundaries (ALIGNED), the offset of the first byte, which the lanes of a row
+// share.
+template <typename Tin, bool ALIGNED>
+struct Raw8 {
+  static constexpr int kVecs = int(sizeof(Tin)) / 2 + (ALIGNED ? 0 : 1);
+  uint4 w[kVecs];
+
+  __device__ __forceinline__ void load(const Tin* p) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint4* base = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-      }
-      return;
-    }
+    for (int i = 0; i < int(sizeof(Tin)) / 2; ++i) w[i] = __ldg(base + i);
+    if constexpr (!ALIGNED)
+      w[kVecs - 1] = (at & 15) ? __ldg(base + kVecs - 1) : make_uint4(0, 0, 0, 0);
   }
+  __device__ __forceinline__ void values(uint32_t offset, float (&v)[8]) const {
+    constexpr int kIn = 4 * kVecs, kOut = 2 * int(sizeof(Tin));
+    uint32_t x[kIn];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      x[4 * i] = w[i].x, x[4 * i + 1] = w[i].y, x[4 * i + 2] = w[i].z, x[4 * i + 3] = w[i].w;
+    }
+    if constexpr (!ALIGNED) {
+      // a shift by whole words, then by the bytes that are left
+      if (offset & 8) {
+#pragma unroll
+        for (int i = 0; i + 2 < kIn; ++i) x[i] = x[i + 2];
+      }
+      if (offset & 4) {
+#pragma unroll
+        for (int i = 0; i + 1 < kIn; ++i) x[i] = x[i + 1];
+      }
+      if constexpr (sizeof(Tin) == 2) {
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) x[i] = __funnelshift_r(x[i], x[i + 1], 8 * (offset & 3));
+      }
+    }
+    const Tin* e = reinterpret_cast<const Tin*>(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  }
+};
+// Eight consecutive elements, one by one, of which `n` exist (the rest are 0).
+template <typename Tin>
+__device__ __forceinline__ void load8(const Tin* p, int64_t n, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
 }
@@ -69,49 +96,75 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3));
 }
 
-// The factors of x * 448 / amax = (x * num) / den; up keeps den normal.
+// The factors of x * 448 / amax = (x * num) / den; up keeps den, and residuals
+// of quotients down to e4m3's least, out of the subnormal range.
 struct Ratio {
   float num, den;
 };
 __device__ __forceinline__ Ratio ratio_of(float amax) {
   if (!(amax > 0.0f)) return {0.875f, 0.875f};
-  const float up = amax < 0x1p-100f ? 0x1p100f : 1.0f;
+  const float up = amax < 0x1p-60f ? 0x1p100f : 1.0f;
   return {0.875f * up, amax * up * 0x1p-9f};
 }
 __device__ __forceinline__ float fp32_scale(float amax) {
   return amax > 0.0f ? amax / 448.0f : 1.0f;
 }
 
-// Two values over den, rounded to e4m3: by the reciprocal where both its bounds
-// agree, else divided.
-__device__ __forceinline__ uint32_t e4m3x2_over(float a, float b, float den, float inv) {
-  constexpr float kLo = 1.0f - 0x1p-22f, kHi = 1.0f + 0x1p-22f;
-  const float x = a * inv, y = b * inv;
-  uint32_t q = e4m3x2(x * kLo, y * kLo);
-  if (q != e4m3x2(x * kHi, y * kHi)) q = e4m3x2(a / den, b / den);
-  return q;
+// a / den, correctly rounded, from y = 1 / den correctly rounded: q = a y is off
+// by an ulp at most, the residual a - q den is exact in one fma, and q + residual
+// * y then rounds to the quotient (P. Markstein's theorem, 1990). den0 is den, or
+// 0 for an infinite den, whose finite quotients are q = 0.
+__device__ __forceinline__ float quotient(float a, float den0, float y) {
+  const float q = a * y;
+  return fmaf(fmaf(-q, den0, a), y, q);
 }
 
 // ITERS: runs of 256 columns per warp. One row's warps follow one another.
-template <typename Tin, bool VEC, bool GATED, bool UE8M0, int ITERS>
+template <typename Tin, bool ALIGNED, bool GATED, bool UE8M0, int ITERS>
 __global__ void __launch_bounds__(32 * kRowWarps)
     fp8_quantize_rows_kernel(const QuantRows p, uint32_t chunks) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
-  const int64_t unit = int64_t(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+  const uint32_t unit = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   const int64_t t = unit / chunks;
   if (t >= p.T) return;
-  const int64_t c0 = int64_t(uint32_t(unit - t * chunks)) * (256 * ITERS) + 8 * lane;
+  const int64_t c0 = int64_t(unit - uint32_t(t) * chunks) * (256 * ITERS) + 8 * lane;
   const Tin* row = static_cast<const Tin*>(p.x) + t * p.ld_x;
   float v[ITERS][8];
   float u[GATED ? ITERS : 1][8];
+  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
+  const uint32_t off_u = uint32_t(reinterpret_cast<uintptr_t>(row + p.K)) & 15u;
+  Raw8<Tin, ALIGNED> raw[ITERS], raw_u[GATED ? ITERS : 1];
+  // one branch for the warp, not one per load: the loads go out together
+  const bool whole = c0 - 8 * lane + 256 * ITERS <= p.K;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    const int64_t c = c0 + 256 * i;
-    const int n = int(min(int64_t(8), max(int64_t(0), p.K - c)));
-    load8<Tin, VEC>(row + c, n, v[i]);
-    if constexpr (GATED) load8<Tin, VEC>(row + p.K + c, n, u[i]);
+    for (int i = 0; i < ITERS; ++i) {
+      raw[i].load(row + c0 + 256 * i);
+      if constexpr (GATED) raw_u[i].load(row + p.K + c0 + 256 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      raw[i].values(off, v[i]);
+      if constexpr (GATED) raw_u[i].values(off_u, u[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int64_t c = c0 + 256 * i;
+      if (c + 8 <= p.K) {
+        raw[0].load(row + c);
+        raw[0].values(off, v[i]);
+        if constexpr (GATED) {
+          raw_u[0].load(row + p.K + c);
+          raw_u[0].values(off_u, u[i]);
+        }
+      } else {
+        load8(row + c, p.K - c, v[i]);
+        if constexpr (GATED) load8(row + p.K + c, p.K - c, u[i]);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
@@ -159,10 +212,11 @@ __global__ void __launch_bounds__(32 * kRowWarps)
       if (writer) static_cast<uint8_t*>(p.scale)[t * p.s_row + blk * p.s_blk] = uint8_t(b);
     } else {
       const Ratio r = ratio_of(amax);
-      const float inv = 1.0f / r.den;
+      const float inv = 1.0f / r.den, den0 = amax < INFINITY ? r.den : 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        w[e] = e4m3x2_over(v[i][2 * e] * r.num, v[i][2 * e + 1] * r.num, r.den, inv);
+        w[e] = e4m3x2(quotient(v[i][2 * e] * r.num, den0, inv),
+                      quotient(v[i][2 * e + 1] * r.num, den0, inv));
       if (writer) static_cast<float*>(p.scale)[t * p.s_row + blk * p.s_blk] = fp32_scale(amax);
     }
     // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
@@ -222,40 +276,40 @@ __global__ void __launch_bounds__(32 * kBlkWarps)
     }
 }
 
-template <typename Tin, bool VEC, bool GATED, int ITERS>
+template <typename Tin, bool ALIGNED, bool GATED, int ITERS>
 int launch_rows_i(const QuantRows& p, int ue8m0, cudaStream_t s) {
   const int64_t chunks = ceil_div(p.K, 256 * ITERS);
   const int64_t blocks = ceil_div(p.T * chunks, kRowWarps);
-  KSW_REQUIRE(blocks < (int64_t(1) << 31), MOE_ERR_UNSUPPORTED,
-              "fp8_quantize_rows: too many blocks");
+  KSW_REQUIRE(blocks * kRowWarps < (int64_t(1) << 32), MOE_ERR_UNSUPPORTED,
+              "fp8_quantize_rows: too many elements");
   if (ue8m0)
-    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, true, ITERS>, dim3(unsigned(blocks)),
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, ALIGNED, GATED, true, ITERS>, dim3(unsigned(blocks)),
                dim3(32 * kRowWarps), 0, s, p, uint32_t(chunks));
   else
-    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, VEC, GATED, false, ITERS>, dim3(unsigned(blocks)),
+    KSW_LAUNCH(fp8_quantize_rows_kernel<Tin, ALIGNED, GATED, false, ITERS>, dim3(unsigned(blocks)),
                dim3(32 * kRowWarps), 0, s, p, uint32_t(chunks));
   return MOE_OK;
 }
 
-template <typename Tin, bool VEC, bool GATED>
+template <typename Tin, bool ALIGNED, bool GATED>
 int launch_rows(const QuantRows& p, int ue8m0, cudaStream_t s) {
   // 256 columns per warp until the SMs are full of warps, then more loads in
   // flight per warp
   constexpr int kMany = GATED || sizeof(Tin) == 4 ? 2 : 4;
-  if (p.T * ceil_div(p.K, 256) <= 148 * 64) return launch_rows_i<Tin, VEC, GATED, 1>(p, ue8m0, s);
-  return launch_rows_i<Tin, VEC, GATED, kMany>(p, ue8m0, s);
+  if (p.T * ceil_div(p.K, 256) <= 148 * 64)
+    return launch_rows_i<Tin, ALIGNED, GATED, 1>(p, ue8m0, s);
+  return launch_rows_i<Tin, ALIGNED, GATED, kMany>(p, ue8m0, s);
 }
 
 template <typename Tin>
 int launch_rows_t(const QuantRows& p, int gated, int ue8m0, cudaStream_t s) {
-  // 16-byte loads when every row, and the up half, starts on such a boundary
-  const bool vec = aligned16(p.x) && (p.ld_x * sizeof(Tin)) % 16 == 0 &&
-                   (!gated || (p.K * sizeof(Tin)) % 16 == 0);
+  const bool aligned = aligned16(p.x) && (p.ld_x * sizeof(Tin)) % 16 == 0 &&
+                       (!gated || (p.K * sizeof(Tin)) % 16 == 0);
   if (gated)
-    return vec ? launch_rows<Tin, true, true>(p, ue8m0, s)
-               : launch_rows<Tin, false, true>(p, ue8m0, s);
-  return vec ? launch_rows<Tin, true, false>(p, ue8m0, s)
-             : launch_rows<Tin, false, false>(p, ue8m0, s);
+    return aligned ? launch_rows<Tin, true, true>(p, ue8m0, s)
+                   : launch_rows<Tin, false, true>(p, ue8m0, s);
+  return aligned ? launch_rows<Tin, true, false>(p, ue8m0, s)
+                 : launch_rows<Tin, false, false>(p, ue8m0, s);
 }
 
 template <typename Tin>
