@@ -36,6 +36,7 @@ struct BalanceParams {
   int64_t T;
   int E, k, G, EG, kept;
   uint32_t eg_magic;  // ceil(2^22 / EG): e / EG = (e * eg_magic) >> 22 for e < 1024, EG <= 1024
+  int lanes_per_group;  // the largest power of two with G * lanes_per_group <= 32
   int softmax, top2, renorm;
   float scale;
   void* weights;
@@ -49,13 +50,9 @@ __device__ __forceinline__ uint32_t group_of(const BalanceParams& p, int e) {
   return (uint32_t(e) * p.eg_magic) >> 22;
 }
 
-// Largest value of a 32-bit key over the warp, and the smallest index among
-// the lanes that hold it.
+// Largest value of a 32-bit key over the warp.
 __device__ __forceinline__ uint32_t redux_max(uint32_t v) {
   return __reduce_max_sync(0xffffffffu, v);
-}
-__device__ __forceinline__ uint32_t redux_min(uint32_t v) {
-  return __reduce_min_sync(0xffffffffu, v);
 }
 // Order-preserving map of floats to unsigned integers; 0 is below all of them.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -64,38 +61,6 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
-// The warp's best (value, index): larger value, then lower index; lanes
-// with i == INT32_MAX have nothing to offer.
-__device__ __forceinline__ void warp_best(float& v, int& i) {
-  const uint32_t key = i == INT32_MAX ? 0u : order_key(v);
-  const uint32_t best = redux_max(key);
-  i = int(redux_min(key == best ? uint32_t(i) : uint32_t(INT32_MAX)));
-  v = key_value(best);
-}
-__device__ __forceinline__ void warp_best(double& v, int& i) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double ov = __shfl_xor_sync(0xffffffffu, v, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, i, o);
-    const bool take = oi != INT32_MAX && (i == INT32_MAX || ov > v || (ov == v && oi < i));
-    if (take) {
-      v = ov;
-      i = oi;
-    }
-  }
-}
-
-template <typename R>
-__device__ __forceinline__ R real_exp(R x);
-template <>
-__device__ __forceinline__ float real_exp<float>(float x) {
-  return expf(x);
-}
-template <>
-__device__ __forceinline__ double real_exp<double>(double x) {
-  return exp(x);
 }
 
 template <typename R>
@@ -111,107 +76,169 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Error bound of the difference of two 32-bit c (per unit of the row's
-// largest score, and of |c|): expf is off by 2 ulp at most, the sigmoid's add
-// and divide by half a one each, the softmax's sum of up to 1024 terms by
-// 37 / 2 ulp in the worst case; the sum with the bias rounds once more.
-constexpr float kTolScore = 4e-6f, kTolValue = 4e-7f;
+// The 32-bit scores that the choice is first made by: fast exponentials and
+// reciprocals, whose errors the choice allows for. CUDA documents at most 2 +
+// 1.173 |x| ulp for __expf(x) and 2 ulp for __fdividef.
+__device__ __forceinline__ float score_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double score_exp(double x) { return exp(x); }
+__device__ __forceinline__ float score_div(float a, float b) { return __fdividef(a, b); }
+__device__ __forceinline__ double score_div(double a, double b) { return a / b; }
 
-// Selects the row's experts in the arithmetic of R. Lane s < k returns the
-// s-th expert in `sel`. Returns (32 bits only) whether some comparison was
-// too close to trust. `mx` is the row's largest logit; `scratch` holds E + G
-// values of R for this warp (groups only).
+// Error bound of one 32-bit score, per unit of the row's largest, in ulp (2^-23).
+// Sigmoid: exp's error counts (1 - s) times; s (1 - s) |x| is under 0.23 for
+// positive logits, and for negative ones s is e^l to first order, so that 2 +
+// 1.173 |l| counts at the largest logit (below it s falls faster than |l|
+// grows); the add and the division 2.5. Softmax: e^-d (2 + 1.173 d) <= 2.5 for
+// exp, the division 2.5, and the error of the sum, which the terms at distance d
+// share in by their weight: their mean d is at most ln 1024 < 7, so 10.2 for
+// the terms, and half an ulp for each of the PL + 4 additions.
+template <int PL>
+__device__ __forceinline__ float score_ulps(int softmax, float mx) {
+  return softmax ? 16.0f + 0.5f * (PL + 4) : 6.0f + 1.2f * fmaxf(-mx, 0.0f);
+}
+
+// c of the row's experts, lane l's j-th being expert l + 32 j. `mx` is the
+// row's largest logit; a NaN ranks last. `smax` returns the largest score.
 template <typename R, int PL, typename Tin>
-__device__ bool select_row(const BalanceParams& p, const Tin* row, const float (&l)[PL], float mx,
-                           int lane, R* scratch, int& sel) {
-  constexpr bool kSingle = std::is_same<R, float>::value;
-  R c[PL];
-  R sum = R(0);
+__device__ __forceinline__ void biased_scores(const BalanceParams& p, const float (&l)[PL],
+                                              float mx, int lane, R (&c)[PL], R& smax) {
   const R rmx = mx == -INFINITY ? R(0) : R(mx);
+  float b[PL];
+#pragma unroll
+  for (int j = 0; j < PL; ++j)
+    b[j] = p.bias != nullptr ? __ldg(p.bias + min(lane + 32 * j, p.E - 1)) : 0.0f;
   if (p.softmax) {
+    R sum = R(0);
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-      c[j] = real_exp(R(l[j]) - rmx);
+      c[j] = score_exp(R(l[j]) - rmx);
       if (lane + 32 * j < p.E) sum += c[j];
     }
     sum = warp_sum(sum);
+    const bool none = mx == -INFINITY;  // no expert has a score: all 0
+    smax = none ? R(0) : score_div(R(1), sum);
+#pragma unroll
+    for (int j = 0; j < PL; ++j) c[j] = none ? R(0) : score_div(c[j], sum);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PL; ++j) c[j] = score_div(R(1), R(1) + score_exp(-R(l[j])));
+    smax = mx == -INFINITY ? R(0) : score_div(R(1), R(1) + score_exp(-rmx));
   }
-  const bool empty = p.softmax && mx == -INFINITY;  // no expert has a score
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    const R v = c[j] + R(b[j]);
+    c[j] = v != v ? R(-INFINITY) : v;
+  }
+}
+
+// Bit g: group g is kept. Sets `close` when the choice hung on less than `tol`
+// (given the value of the last group kept).
+template <typename R, int PL, typename Tol>
+__device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R (&c)[PL],
+                                                int lane, R* scratch, Tol tol, bool& close) {
+  // position e + group keeps lanes of different groups on different banks
+  __syncwarp();
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
     const int e = lane + 32 * j;
-    const R s = p.softmax ? (empty ? R(0) : c[j] / sum) : R(1) / (R(1) + real_exp(-R(l[j])));
-    R v = s + (p.bias != nullptr && e < p.E ? R(__ldg(p.bias + e)) : R(0));
-    c[j] = v != v ? R(-INFINITY) : v;  // a NaN ranks last
+    if (e < p.E) scratch[e + group_of(p, e)] = c[j];
   }
-  float smax = 0.0f;  // the row's largest score, for the error bound
-  if constexpr (kSingle)
-    smax = p.softmax ? (empty ? 0.0f : 1.0f / sum) : 1.0f / (1.0f + expf(-mx));
-  bool close = false;
+  __syncwarp();
+  const int per = p.lanes_per_group;
+  const int g = lane / per, sub = lane % per;
+  R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
+  if (g < p.G) {
+    const R* at = scratch + g * (p.EG + 1);
+    for (int i = sub; i < p.EG; i += per) {
+      const R v = at[i];
+      b = v > a ? a : (v > b ? v : b);
+      a = v > a ? v : a;
+    }
+  }
+  for (int o = per >> 1; o > 0; o >>= 1) {
+    const R oa = __shfl_xor_sync(0xffffffffu, a, o);
+    const R ob = __shfl_xor_sync(0xffffffffu, b, o);
+    const R lo = a > oa ? oa : a;
+    const R hb = b > ob ? b : ob;
+    a = a > oa ? a : oa;
+    b = lo > hb ? lo : hb;
+  }
+  R value = p.top2 && p.EG > 1 ? a + b : a;  // a group of one has no second
+  if (value != value) value = R(-INFINITY);  // +inf and -inf in one group
+  // a group's rank: how many come before it
+  int rank = 0;
+  for (int h = 0; h < p.G; ++h) {
+    const R o = __shfl_sync(0xffffffffu, value, h * per);
+    rank += o > value || (o == value && h < g);
+  }
+  const bool mine = g < p.G && sub == 0;
+  const bool keep = mine && rank < p.kept;
+  const R last =
+      __shfl_sync(0xffffffffu, value,
+                  __ffs(__ballot_sync(0xffffffffu, mine && rank == p.kept - 1)) - 1);
+  close = mine && !keep && value >= last - tol(last) && last > R(-INFINITY);
+  // ballot bit g * per -> bit g
+  const uint32_t at = __ballot_sync(0xffffffffu, keep);
+  uint32_t kept = 0;
+  for (int h = 0; h < p.G; ++h) kept |= ((at >> (h * per)) & 1u) << h;
+  return kept;
+}
 
-  uint32_t kept = 0xffffffffu;
-  if (p.G > 1) {
-    // position e + group keeps lanes of different groups on different banks
-    __syncwarp();
+// Puts n <= 32 candidates (lane i < n: expert `e`) in their order in 64 bits and
+// returns the first k, lane s the s-th. `list` holds 32 indexes for this warp.
+// Out of the kernel's body, whose registers it would double: few rows need it.
+template <typename Tin>
+__device__ __noinline__ int order_exact(const BalanceParams& p, const Tin* row, float mx, int lane,
+                                        int n, int e, int* list) {
+  double c = -INFINITY;
+  double sum = 0.0;
+  const bool none = mx == -INFINITY;
+  if (p.softmax && !none) {
+    for (int i = lane; i < p.E; i += 32) sum += exp(double(to_f32(row[i])) - double(mx));
+    sum = warp_sum(sum);
+  }
+  if (lane < n) {
+    const double l = to_f32(row[e]);
+    const double s = p.softmax ? (none ? 0.0 : exp(l - double(mx)) / sum) : 1.0 / (1.0 + exp(-l));
+    c = s + (p.bias != nullptr ? double(__ldg(p.bias + e)) : 0.0);
+    if (c != c) c = -INFINITY;
+  }
+  int rank = 0;
+  for (int h = 0; h < n; ++h) {
+    const double oc = __shfl_sync(0xffffffffu, c, h);
+    const int oe = __shfl_sync(0xffffffffu, e, h);
+    rank += oc > c || (oc == c && oe < e);
+  }
+  if (lane < n) list[rank] = e;
+  __syncwarp();
+  const int sel = lane < p.k ? list[lane] : 0;
+  __syncwarp();
+  return sel;
+}
+
+// The row's experts in 64 bits, groups included: lane s < k returns the s-th.
+template <int PL, typename Tin>
+__device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row, float mx,
+                                         int lane, double* scratch) {
+  float l[PL];
 #pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int e = lane + 32 * j;
-      if (e < p.E) scratch[e + group_of(p, e)] = c[j];
-    }
-    __syncwarp();
-    int per = 32;  // lanes per group: the largest power of two that fits
-    while (per * p.G > 32) per >>= 1;
-    const int g = lane / per, sub = lane % per;
-    R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
-    if (g < p.G) {
-      const R* at = scratch + g * (p.EG + 1);
-      for (int i = sub; i < p.EG; i += per) {
-        const R v = at[i];
-        b = v > a ? a : (v > b ? v : b);
-        a = v > a ? v : a;
-      }
-    }
-    for (int o = per >> 1; o > 0; o >>= 1) {
-      const R oa = __shfl_xor_sync(0xffffffffu, a, o);
-      const R ob = __shfl_xor_sync(0xffffffffu, b, o);
-      const R lo = a > oa ? oa : a;
-      const R hb = b > ob ? b : ob;
-      a = a > oa ? a : oa;
-      b = lo > hb ? lo : hb;
-    }
-    // every lane of the group has its two largest; a group of one has no second
-    R value = p.top2 && p.EG > 1 ? a + b : a;
-    if (value != value) value = R(-INFINITY);  // +inf and -inf in one group
-    const bool mine = g < p.G && sub == 0;
-    kept = 0;
-    bool taken = false;
-    R last = R(0);
-    for (int s = 0; s < p.kept; ++s) {
-      R v = value;
-      int i = mine && !taken ? g : INT32_MAX;
-      warp_best(v, i);
-      kept |= 1u << i;
-      if (mine && g == i) taken = true;
-      last = v;
-    }
-    if constexpr (kSingle) {
-      const float tol = 2.0f * (kTolScore * smax + kTolValue * fabsf(last));
-      close = mine && !taken && value >= last - tol && last > -INFINITY;
-    }
-  }
-
+  for (int j = 0; j < PL; ++j)
+    l[j] = lane + 32 * j < p.E ? to_f32(row[lane + 32 * j]) : -INFINITY;
+  double c[PL], smax;
+  biased_scores<double, PL, Tin>(p, l, mx, lane, c, smax);
+  uint32_t kept = 0xffffffffu;
+  bool close = false;
+  if (p.G > 1)
+    kept = kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
   uint32_t open = 0;  // bit j: expert lane + 32 j may still be chosen
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
     const int e = lane + 32 * j;
-    const uint32_t g = p.G > 1 ? group_of(p, e) : 0u;
-    if (e < p.E && ((kept >> g) & 1u)) open |= 1u << j;
+    if (e < p.E && (p.G == 1 || ((kept >> group_of(p, e)) & 1u))) open |= 1u << j;
   }
-  sel = 0;
-  R last = R(0);
-  float last_l = 0.0f, last_b = 0.0f;
+  int sel = 0;
   for (int s = 0; s < p.k; ++s) {
-    R v = R(-INFINITY);
+    double v = -INFINITY;
     int i = INT32_MAX;
 #pragma unroll
     for (int j = 0; j < PL; ++j)
@@ -219,40 +246,125 @@ __device__ bool select_row(const BalanceParams& p, const Tin* row, const float (
         v = c[j];
         i = lane + 32 * j;
       }
-    warp_best(v, i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const double ov = __shfl_xor_sync(0xffffffffu, v, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, i, o);
+      if (oi != INT32_MAX && (i == INT32_MAX || ov > v || (ov == v && oi < i))) {
+        v = ov;
+        i = oi;
+      }
+    }
     if ((i & 31) == lane) open &= ~(1u << (i >> 5));
     if (lane == s) sel = i;
-    if constexpr (kSingle) {
-      // the pick's logit and bias: uniform loads of what the warp has read
-      const float li = to_f32(row[i]);
-      const float bi = p.bias != nullptr ? __ldg(p.bias + i) : 0.0f;
-      if (s > 0 && last - v <= kTolScore * smax + kTolValue * fabsf(last) &&
-          !(li == last_l && bi == last_b))
-        close = true;
-      last_l = li;
-      last_b = bi;
-    }
-    last = v;
   }
-  if constexpr (kSingle) {
-    // the experts left out must be clear of the last one chosen
-    const float bar = last - (kTolScore * smax + kTolValue * fabsf(last));
+  return sel;
+}
+
+// Whether two experts tie in truth: equal logits and equal biases.
+template <typename Tin>
+__device__ __forceinline__ bool true_tie(const BalanceParams& p, const Tin* row, int a, int b) {
+  return to_f32(row[a]) == to_f32(row[b]) &&
+         (p.bias == nullptr || __ldg(p.bias + a) == __ldg(p.bias + b));
+}
+
+// The same in 32 bits; a row some of whose comparisons were too close to trust
+// goes on in 64: the chosen and those within the tolerance of the last one,
+// or the whole row where a group's place was in doubt. The values are held as ordered unsigned keys whose low
+// bits give way to the lane's index of the expert (PL - 1 - j, so that ties go to
+// the lower one), 0 for one that cannot be chosen. Each lane sorts its keys; a
+// pick is the warp-wide maximum of the lanes' first keys, popped in its lane.
+template <int PL, typename Tin>
+__device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row,
+                                          const float (&l)[PL], float mx, int lane,
+                                          double* scratch, int* list) {
+  float c[PL], smax;
+  biased_scores<float, PL, Tin>(p, l, mx, lane, c, smax);
+  // of a difference of two c: both scores, the rounding of both sums with the
+  // bias and the bits cut off both keys; twice that, since it is itself rounded
+  const float scores = 2.0f * 2.0f * score_ulps<PL>(p.softmax, mx) * 0x1p-23f * smax;
+  auto tol = [&](float v) { return scores + 2.0f * 2.0f * (PL + 0.5f) * 0x1p-23f * fabsf(v); };
+  uint32_t kept = 0xffffffffu;
+  if (p.G > 1) {
+    bool close = false;
+    kept = kept_groups(p, c, lane, reinterpret_cast<float*>(scratch),
+                       [&](float v) { return 2.0f * tol(v); }, close);
+    if (__any_sync(0xffffffffu, close)) return select_exact<PL>(p, row, mx, lane, scratch);
+  }
+  constexpr uint32_t kLow = PL - 1;
+  uint32_t key[PL];
 #pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int e = lane + 32 * j;
-      if (((open >> j) & 1u) && c[j] >= bar && last > -INFINITY &&
-          !(l[j] == last_l && (p.bias == nullptr || __ldg(p.bias + e) == last_b)))
-        close = true;
-    }
-    return __any_sync(0xffffffffu, close);
+  for (int j = 0; j < PL; ++j) {
+    const int e = lane + 32 * j;
+    const bool in = e < p.E && (p.G == 1 || ((kept >> group_of(p, e)) & 1u));
+    key[j] = in ? (order_key(c[j]) & ~kLow) | (kLow - j) : 0u;
   }
-  return false;
+  // bitonic sort, descending
+#pragma unroll
+  for (int w = 2; w <= PL; w <<= 1)
+#pragma unroll
+    for (int d = w >> 1; d > 0; d >>= 1)
+#pragma unroll
+      for (int j = 0; j < PL; ++j)
+        if ((j ^ d) > j) {
+          const uint32_t lo = min(key[j], key[j ^ d]), hi = max(key[j], key[j ^ d]);
+          const bool down = (j & w) == 0;
+          key[j] = down ? hi : lo;
+          key[j ^ d] = down ? lo : hi;
+        }
+  int sel = 0, last_i = 0;
+  float last = 0.0f;
+  bool close = false;
+  for (int s = 0; s < p.k; ++s) {
+    const uint32_t best = redux_max(key[0]);
+    const int src = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+    const int i = src + 32 * int(kLow - (best & kLow));
+    if (lane == s) sel = i;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) key[j] = lane != src ? key[j] : j + 1 < PL ? key[j + 1] : 0u;
+    const float v = key_value(best & ~kLow);
+    if (s > 0 && last - v <= tol(last) && !true_tie(p, row, last_i, i)) close = true;
+    last = v;
+    last_i = i;
+  }
+  // the experts left out must be clear of the last one chosen
+  if (last > -INFINITY) {
+    const uint32_t bar = order_key(last - tol(last)) & ~kLow;
+    bool near = false;
+    if (key[0] >= bar) {
+#pragma unroll
+      for (int j = 0; j < PL; ++j)
+        near |= key[j] >= bar && key[j] != 0u &&
+                !true_tie(p, row, last_i, lane + 32 * int(kLow - (key[j] & kLow)));
+    }
+    if (__any_sync(0xffffffffu, near) || close) {
+      int n = p.k;
+      if (lane < p.k) list[lane] = sel;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) {
+        const bool in = key[j] >= bar && key[j] != 0u;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        const int at = n + __popc(who & lanemask_lt());
+        if (in && at < 32) list[at] = lane + 32 * int(kLow - (key[j] & kLow));
+        n += __popc(who);
+      }
+      __syncwarp();
+      const int e = list[lane];
+      __syncwarp();
+      return n <= 32 ? order_exact(p, row, mx, lane, n, e, list)
+                     : select_exact<PL>(p, row, mx, lane, scratch);
+    }
+  } else if (close) {
+    return select_exact<PL>(p, row, mx, lane, scratch);
+  }
+  return sel;
 }
 
 template <int PL, typename Tin>
-__global__ void __launch_bounds__(32 * kMaxWarps)
+__global__ void __launch_bounds__(32 * kMaxWarps, PL <= 8 ? 8 : 4)
     balanced_topk_kernel(const BalanceParams p) {
   extern __shared__ double s_scratch[];
+  __shared__ int s_list[kMaxWarps][32];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -269,9 +381,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
       mx = fmaxf(mx, l[j]);
     }
     mx = warp_max(mx);
-    int sel;
-    if (select_row<float, PL>(p, row, l, mx, lane, reinterpret_cast<float*>(scratch), sel))
-      select_row<double, PL>(p, row, l, mx, lane, scratch, sel);
+    const int sel = select_row<PL>(p, row, l, mx, lane, scratch, s_list[warp]);
 
     // weights of the chosen: lane s < k has the s-th
     const bool mine = lane < p.k;
@@ -496,6 +606,8 @@ extern "C" int moe_balanced_topk(const void* router_logits, int logits_dtype,
   p.EG = num_experts / num_expert_group;
   p.kept = topk_group;
   p.eg_magic = uint32_t(((1 << 22) + p.EG - 1) / p.EG);
+  p.lanes_per_group = 32;
+  while (p.lanes_per_group * p.G > 32) p.lanes_per_group >>= 1;
   p.softmax = scoring_func == 0;
   p.top2 = group_score;
   p.renorm = renormalize;
