@@ -37,6 +37,7 @@ struct BalanceParams {
   int E, k, G, EG, kept;
   uint32_t eg_magic;  // ceil(2^22 / EG): e / EG = (e * eg_magic) >> 22 for e < 1024, EG <= 1024
   int lanes_per_group;  // the largest power of two with G * lanes_per_group <= 32
+  int group_shift;      // its logarithm
   int softmax, top2, renorm;
   float scale;
   void* weights;
@@ -57,7 +58,7 @@ __device__ __forceinline__ uint32_t redux_max(uint32_t v) {
 // Order-preserving map of floats to unsigned integers; 0 is below all of them.
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t u = __float_as_uint(v);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
@@ -77,21 +78,32 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // The 32-bit scores that the choice is first made by: fast exponentials and
-// reciprocals, whose errors the choice allows for. CUDA documents at most 2 +
-// 1.173 |x| ulp for __expf(x) and 2 ulp for __fdividef.
-__device__ __forceinline__ float score_exp(float x) { return __expf(x); }
+// reciprocals, whose errors the choice allows for. The PTX manual gives 2^-22 for
+// ex2.approx and 1 ulp for rcp.approx; the argument's product with log2(e) is
+// off by half an ulp of itself, |x| * 2^-24 in the result's relative error, and
+// as much again through the constant.
+__device__ __forceinline__ float score_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
 __device__ __forceinline__ double score_exp(double x) { return exp(x); }
-__device__ __forceinline__ float score_div(float a, float b) { return __fdividef(a, b); }
-__device__ __forceinline__ double score_div(double a, double b) { return a / b; }
+__device__ __forceinline__ float score_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ double score_rcp(double x) { return 1.0 / x; }
 
-// Error bound of one 32-bit score, per unit of the row's largest, in ulp (2^-23).
-// Sigmoid: exp's error counts (1 - s) times; s (1 - s) |x| is under 0.23 for
-// positive logits, and for negative ones s is e^l to first order, so that 2 +
-// 1.173 |l| counts at the largest logit (below it s falls faster than |l|
-// grows); the add and the division 2.5. Softmax: e^-d (2 + 1.173 d) <= 2.5 for
-// exp, the division 2.5, and the error of the sum, which the terms at distance d
-// share in by their weight: their mean d is at most ln 1024 < 7, so 10.2 for
-// the terms, and half an ulp for each of the PL + 4 additions.
+// Error bound of one 32-bit score, per unit of the row's largest, in ulp (2^-23);
+// exp(x) is off by 2 + |x|. Sigmoid: exp's error counts (1 - s) times; s (1 - s)
+// |x| is under 0.23 for positive logits, and for negative ones s is e^l to first
+// order, so that 2 + |l| counts at the largest logit (below it s falls faster
+// than |l| grows); the add and the reciprocal 1.5. Softmax: e^-d (2 + d) <= 2 for
+// exp, the difference l - max 0.2, the reciprocal and the product 1.5, and the
+// error of the sum, which the terms at distance d share in by their weight: their
+// mean d is at most ln 1024 < 7, so 9 for the terms, and half an ulp for each of
+// the PL + 4 additions.
 template <int PL>
 __device__ __forceinline__ float score_ulps(int softmax, float mx) {
   return softmax ? 16.0f + 0.5f * (PL + 4) : 6.0f + 1.2f * fmaxf(-mx, 0.0f);
@@ -116,13 +128,13 @@ __device__ __forceinline__ void biased_scores(const BalanceParams& p, const floa
     }
     sum = warp_sum(sum);
     const bool none = mx == -INFINITY;  // no expert has a score: all 0
-    smax = none ? R(0) : score_div(R(1), sum);
+    smax = none ? R(0) : score_rcp(sum);
 #pragma unroll
-    for (int j = 0; j < PL; ++j) c[j] = none ? R(0) : score_div(c[j], sum);
+    for (int j = 0; j < PL; ++j) c[j] = none ? R(0) : c[j] * smax;
   } else {
 #pragma unroll
-    for (int j = 0; j < PL; ++j) c[j] = score_div(R(1), R(1) + score_exp(-R(l[j])));
-    smax = mx == -INFINITY ? R(0) : score_div(R(1), R(1) + score_exp(-rmx));
+    for (int j = 0; j < PL; ++j) c[j] = score_rcp(R(1) + score_exp(-R(l[j])));
+    smax = mx == -INFINITY ? R(0) : score_rcp(R(1) + score_exp(-rmx));
   }
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
@@ -131,8 +143,18 @@ __device__ __forceinline__ void biased_scores(const BalanceParams& p, const floa
   }
 }
 
-// Bit g: group g is kept. Sets `close` when the choice hung on less than `tol`
-// (given the value of the last group kept).
+// Two largest of (a >= b) and v.
+__device__ __forceinline__ void top_two(float v, float& a, float& b) {
+  b = fmaxf(b, fminf(a, v));
+  a = fmaxf(a, v);
+}
+__device__ __forceinline__ void top_two(double v, double& a, double& b) {
+  b = fmax(b, fmin(a, v));
+  a = fmax(a, v);
+}
+
+// Bit g * lanes_per_group: group g is kept. Sets `close` when the choice hung on
+// less than `tol` (given the value of the last group kept).
 template <typename R, int PL, typename Tol>
 __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R (&c)[PL],
                                                 int lane, R* scratch, Tol tol, bool& close) {
@@ -145,23 +167,18 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
   }
   __syncwarp();
   const int per = p.lanes_per_group;
-  const int g = lane / per, sub = lane % per;
+  const int g = lane >> p.group_shift, sub = lane & (per - 1);
   R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
   if (g < p.G) {
     const R* at = scratch + g * (p.EG + 1);
-    for (int i = sub; i < p.EG; i += per) {
-      const R v = at[i];
-      b = v > a ? a : (v > b ? v : b);
-      a = v > a ? v : a;
-    }
+#pragma unroll 4
+    for (int i = sub; i < p.EG; i += per) top_two(at[i], a, b);
   }
   for (int o = per >> 1; o > 0; o >>= 1) {
     const R oa = __shfl_xor_sync(0xffffffffu, a, o);
     const R ob = __shfl_xor_sync(0xffffffffu, b, o);
-    const R lo = a > oa ? oa : a;
-    const R hb = b > ob ? b : ob;
-    a = a > oa ? a : oa;
-    b = lo > hb ? lo : hb;
+    top_two(oa, a, b);
+    top_two(ob, a, b);
   }
   R value = p.top2 && p.EG > 1 ? a + b : a;  // a group of one has no second
   if (value != value) value = R(-INFINITY);  // +inf and -inf in one group
@@ -177,11 +194,10 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
       __shfl_sync(0xffffffffu, value,
                   __ffs(__ballot_sync(0xffffffffu, mine && rank == p.kept - 1)) - 1);
   close = mine && !keep && value >= last - tol(last) && last > R(-INFINITY);
-  // ballot bit g * per -> bit g
-  const uint32_t at = __ballot_sync(0xffffffffu, keep);
-  uint32_t kept = 0;
-  for (int h = 0; h < p.G; ++h) kept |= ((at >> (h * per)) & 1u) << h;
-  return kept;
+  return __ballot_sync(0xffffffffu, keep);
+}
+__device__ __forceinline__ bool is_kept(const BalanceParams& p, uint32_t kept, int e) {
+  return p.G == 1 || ((kept >> (group_of(p, e) << p.group_shift)) & 1u);
 }
 
 // Puts n <= 32 candidates (lane i < n: expert `e`) in their order in 64 bits and
@@ -216,25 +232,42 @@ __device__ __noinline__ int order_exact(const BalanceParams& p, const Tin* row, 
   return sel;
 }
 
-// The row's experts in 64 bits, groups included: lane s < k returns the s-th.
+// c of the row in 64 bits, from its logits in memory.
 template <int PL, typename Tin>
-__device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row, float mx,
-                                         int lane, double* scratch) {
+__device__ __forceinline__ void exact_scores(const BalanceParams& p, const Tin* row, float mx,
+                                             int lane, double (&c)[PL]) {
   float l[PL];
 #pragma unroll
   for (int j = 0; j < PL; ++j)
     l[j] = lane + 32 * j < p.E ? to_f32(row[lane + 32 * j]) : -INFINITY;
-  double c[PL], smax;
+  double smax;
   biased_scores<double, PL, Tin>(p, l, mx, lane, c, smax);
+}
+
+// The groups kept, in 64 bits (is_kept's mask).
+template <int PL, typename Tin>
+__device__ __noinline__ uint32_t kept_exact(const BalanceParams& p, const Tin* row, float mx,
+                                            int lane, double* scratch) {
+  double c[PL];
+  exact_scores<PL>(p, row, mx, lane, c);
+  bool close = false;
+  return kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
+}
+
+// The row's experts in 64 bits, groups included: lane s < k returns the s-th.
+template <int PL, typename Tin>
+__device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row, float mx,
+                                         int lane, double* scratch) {
+  double c[PL];
+  exact_scores<PL>(p, row, mx, lane, c);
   uint32_t kept = 0xffffffffu;
   bool close = false;
-  if (p.G > 1)
-    kept = kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
+  if (p.G > 1) kept = kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
   uint32_t open = 0;  // bit j: expert lane + 32 j may still be chosen
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
     const int e = lane + 32 * j;
-    if (e < p.E && (p.G == 1 || ((kept >> group_of(p, e)) & 1u))) open |= 1u << j;
+    if (e < p.E && is_kept(p, kept, e)) open |= 1u << j;
   }
   int sel = 0;
   for (int s = 0; s < p.k; ++s) {
@@ -269,11 +302,12 @@ __device__ __forceinline__ bool true_tie(const BalanceParams& p, const Tin* row,
 }
 
 // The same in 32 bits; a row some of whose comparisons were too close to trust
-// goes on in 64: the chosen and those within the tolerance of the last one,
-// or the whole row where a group's place was in doubt. The values are held as ordered unsigned keys whose low
-// bits give way to the lane's index of the expert (PL - 1 - j, so that ties go to
-// the lower one), 0 for one that cannot be chosen. Each lane sorts its keys; a
-// pick is the warp-wide maximum of the lanes' first keys, popped in its lane.
+// goes on in 64: the groups where one's place was in doubt, then the chosen and
+// those within the tolerance of the last one. The values are held as ordered
+// unsigned keys whose low bits give way to the lane's index of the expert (PL - 1
+// - j, so that ties go to the lower one), 0 for one that cannot be chosen. Each
+// lane sorts its keys; a pick is the warp-wide maximum of the lanes' first keys,
+// popped in its lane.
 template <int PL, typename Tin>
 __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row,
                                           const float (&l)[PL], float mx, int lane,
@@ -286,17 +320,19 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   auto tol = [&](float v) { return scores + 2.0f * 2.0f * (PL + 0.5f) * 0x1p-23f * fabsf(v); };
   uint32_t kept = 0xffffffffu;
   if (p.G > 1) {
+    // a value is the sum of two uncut c, rounded once more
     bool close = false;
-    kept = kept_groups(p, c, lane, reinterpret_cast<float*>(scratch),
-                       [&](float v) { return 2.0f * tol(v); }, close);
-    if (__any_sync(0xffffffffu, close)) return select_exact<PL>(p, row, mx, lane, scratch);
+    kept = kept_groups(
+        p, c, lane, reinterpret_cast<float*>(scratch),
+        [&](float v) { return 2.0f * scores + 2.0f * 2.0f * 1.5f * 0x1p-23f * fabsf(v); }, close);
+    if (__any_sync(0xffffffffu, close)) kept = kept_exact<PL>(p, row, mx, lane, scratch);
   }
   constexpr uint32_t kLow = PL - 1;
   uint32_t key[PL];
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
     const int e = lane + 32 * j;
-    const bool in = e < p.E && (p.G == 1 || ((kept >> group_of(p, e)) & 1u));
+    const bool in = e < p.E && is_kept(p, kept, e);
     key[j] = in ? (order_key(c[j]) & ~kLow) | (kLow - j) : 0u;
   }
   // bitonic sort, descending
@@ -606,8 +642,9 @@ extern "C" int moe_balanced_topk(const void* router_logits, int logits_dtype,
   p.EG = num_experts / num_expert_group;
   p.kept = topk_group;
   p.eg_magic = uint32_t(((1 << 22) + p.EG - 1) / p.EG);
-  p.lanes_per_group = 32;
-  while (p.lanes_per_group * p.G > 32) p.lanes_per_group >>= 1;
+  p.group_shift = 5;
+  while ((p.G << p.group_shift) > 32) --p.group_shift;
+  p.lanes_per_group = 1 << p.group_shift;
   p.softmax = scoring_func == 0;
   p.top2 = group_score;
   p.renorm = renormalize;
