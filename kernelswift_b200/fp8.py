@@ -25,6 +25,7 @@ from .fused_moe import _check_cuda, _DTYPE_CODE, _enqueue
 _FORMAT = {"fp32": 0, "ue8m0": 1}
 _SCALE_FORMAT = {torch.float32: 0, torch.uint8: 1}
 _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
+_FLOAT_CODE = {t: _DTYPE_CODE[t] for t in _FLOAT}
 
 
 def _round_up(n: int, m: int) -> int:
@@ -45,7 +46,8 @@ def _no_grad_needed(name: str, t: torch.Tensor) -> None:
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """A 2-D tensor whose rows are dense: `t`, or a dense copy."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.numel() == 0:
+    pitch, step = t.stride()
+    if step == 1 and pitch >= t.shape[1] or t.numel() == 0:
         return t
     return t.contiguous()
 
@@ -56,8 +58,8 @@ def _fp8_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.float8_e4m3fn or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D float8_e4m3fn tensor")
     rows, cols = t.shape
-    if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= cols
-            and t.data_ptr() % 16 == 0):
+    pitch, step = t.stride()
+    if step == 1 and pitch % 16 == 0 and pitch >= cols and t.data_ptr() % 16 == 0:
         return t
     q = _empty_fp8(rows, cols, t.device)
     q.view(torch.uint8).copy_(t.view(torch.uint8))
@@ -74,9 +76,7 @@ def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, inde
 
 
 def _addend(addend: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype, index: int):
-    """(pointer, row stride) of the addend, (None, 0) without one."""
-    if addend is None:
-        return None, 0
+    """(pointer, row stride) of the addend."""
     _no_grad_needed("addend", addend)
     if addend.shape != (rows, cols) or addend.dtype != dtype or addend.get_device() != index:
         raise ValueError(f"addend must be a {dtype} [{rows}, {cols}] tensor on the operands' "
@@ -94,27 +94,31 @@ def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = Fa
     [T, ceil(K / 128)], float32 or uint8), the operands of block_matmul: views
     whose row pitch is padded to 16 bytes (q) and 4 (scale bytes); fp32 scales
     lie column by column."""
-    _check_cuda("x", x)
-    _no_grad_needed("x", x)
-    if scale_format not in _FORMAT:
+    index = x.get_device()
+    if index < 0:
+        _check_cuda("x", x)
+    fmt = _FORMAT.get(scale_format)
+    if fmt is None:
         raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
-    if x.dim() != 2 or x.dtype not in _FLOAT or (gated and x.shape[1] % 2):
+    code = _FLOAT_CODE.get(x.dtype)
+    if x.dim() != 2 or code is None or (gated and x.shape[1] % 2):
         raise ValueError("x must be a 2-D f32/f16/bf16 tensor, of an even width when gated")
+    if x.requires_grad:
+        _no_grad_needed("x", x)
     x = _rows_of(x)
-    T = x.shape[0]
-    K = x.shape[1] // 2 if gated else x.shape[1]
+    T, wide = x.shape
+    K = wide // 2 if gated else wide
     if K < 1:
         raise ValueError("x has no columns")
-    dev, kb = x.device, -(-K // 128)
+    dev, kb = x.device, (K + 127) // 128
     q = _empty_fp8(T, K, dev)
-    if scale_format == "fp32":
-        strides, dtype = (1, _round_up(T, 4)), torch.float32
+    if fmt == 0:
+        strides, dtype = (1, (T + 3) // 4 * 4), torch.float32
     else:
-        strides, dtype = (_round_up(kb, 4), 1), torch.uint8
+        strides, dtype = ((kb + 3) // 4 * 4, 1), torch.uint8
     scale = torch.empty_strided((T, kb), strides, dtype=dtype, device=dev)
-    _enqueue("moe_fp8_quantize_rows", x.get_device(), x.data_ptr(), _DTYPE_CODE[x.dtype], T, K,
-             max(x.stride(0), x.shape[1]), gated, _FORMAT[scale_format], q.data_ptr(),
-             _round_up(K, 16), scale.data_ptr(), *strides)
+    _enqueue("moe_fp8_quantize_rows", index, x.data_ptr(), code, T, K, max(x.stride(0), wide),
+             gated, fmt, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), *strides)
     return q, scale
 
 
@@ -156,14 +160,14 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     (bf16, f16 or f32). status: optional int32 device word (moe_read_status).
     """
     index = x.get_device()
-    for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
-        if t.get_device() != index or index < 0:
+    if not index == w.get_device() == x_scale.get_device() == w_scale.get_device() or index < 0:
+        for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
             _check_cuda(name, t)
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        raise ValueError("x, x_scale, w and w_scale must be on one device")
     x, w = _fp8_rows("x", x), _fp8_rows("w", w)
-    (T, K), N = x.shape, w.shape[0]
-    kb, nb = -(-K // 128), -(-N // 128)
-    if w.shape[1] != K or K < 1 or N < 1:
+    (T, K), (N, w_cols) = x.shape, w.shape
+    kb, nb = (K + 127) // 128, (N + 127) // 128
+    if w_cols != K or K < 1 or N < 1:
         raise ValueError(f"w {tuple(w.shape)} does not match x {tuple(x.shape)}")
     fmt = _SCALE_FORMAT.get(x_scale.dtype)
     if fmt is None or w_scale.dtype != x_scale.dtype:
@@ -172,20 +176,21 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         raise ValueError(f"scales must be [{T}, {kb}] and [{nb}, {kb}], got "
                          f"{tuple(x_scale.shape)} and {tuple(w_scale.shape)}")
     if out is None:
-        if out_dtype not in _FLOAT:
+        if out_dtype not in _FLOAT_CODE:
             raise ValueError("out_dtype must be bf16, f16 or f32")
         out = torch.empty(T, N, dtype=out_dtype, device=x.device)
+        ld_out = N
     else:
         out_dtype = out.dtype
         _check_out(out, T, N, out_dtype, index)
-    add_ptr, add_ld = _addend(addend, T, N, out_dtype, index)
+        ld_out = max(out.stride(0), N)
+    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, N, out_dtype, index)
     if not w_scale.is_contiguous():
         w_scale = w_scale.contiguous()
-    pitch = _round_up(K, 16)
+    pitch = (K + 15) // 16 * 16
     _enqueue("moe_fp8_matmul", index, x.data_ptr(), max(x.stride(0), pitch), x_scale.data_ptr(),
-             x_scale.stride(0), x_scale.stride(1), w.data_ptr(), max(w.stride(0), pitch),
-             w_scale.data_ptr(), fmt, T, N, K, add_ptr, add_ld, out.data_ptr(),
-             max(out.stride(0), N), _DTYPE_CODE[out_dtype],
+             *x_scale.stride(), w.data_ptr(), max(w.stride(0), pitch), w_scale.data_ptr(), fmt, T,
+             N, K, add_ptr, add_ld, out.data_ptr(), ld_out, _FLOAT_CODE[out_dtype],
              None if status is None else status.data_ptr())
     return out
 
@@ -217,11 +222,12 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
     held in x's dtype. addend [T, H] in x's dtype (the routed experts' output; it
     may be out) is added before the one rounding of the result. Four launches."""
     index = x.get_device()
-    for name, t in (("x", x), ("w13", w13), ("w13_scale", w13_scale), ("w2", w2),
-                    ("w2_scale", w2_scale)):
-        if t.get_device() != index or index < 0:
+    if (not index == w13.get_device() == w13_scale.get_device() == w2.get_device()
+            == w2_scale.get_device() or index < 0):
+        for name, t in (("x", x), ("w13", w13), ("w13_scale", w13_scale), ("w2", w2),
+                        ("w2_scale", w2_scale)):
             _check_cuda(name, t)
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        raise ValueError("x and the weights with their scales must be on one device")
     _no_grad_needed("x", x)
     if x.dim() != 2 or x.dtype not in _FLOAT or x.shape[1] < 1:
         raise ValueError("x must be a 2-D f32/f16/bf16 tensor")
@@ -233,16 +239,16 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
     fmt = _SCALE_FORMAT.get(w13_scale.dtype)
     if fmt is None or w2_scale.dtype != w13_scale.dtype:
         raise ValueError("w13_scale and w2_scale must both be float32 or both uint8 (UE8M0)")
-    hb, ib = -(-H // 128), -(-inter // 128)
-    if w13_scale.shape != (-(-2 * inter // 128), hb) or w2_scale.shape != (hb, ib):
-        raise ValueError(f"scales must be [{-(-2 * inter // 128)}, {hb}] and [{hb}, {ib}], got "
+    hb, ib, gb = (H + 127) // 128, (inter + 127) // 128, (2 * inter + 127) // 128
+    if w13_scale.shape != (gb, hb) or w2_scale.shape != (hb, ib):
+        raise ValueError(f"scales must be [{gb}, {hb}] and [{hb}, {ib}], got "
                          f"{tuple(w13_scale.shape)} and {tuple(w2_scale.shape)}")
     x = _rows_of(x)
     if out is None:
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     else:
         _check_out(out, T, H, x.dtype, index)
-    add_ptr, add_ld = _addend(addend, T, H, x.dtype, index)
+    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, H, x.dtype, index)
     code = _DTYPE_CODE[x.dtype]
     # of its own: a workspace kept by stream would be shared by captured graphs
     ws = torch.empty(_mlp_workspace_bytes(T, H, inter, code, fmt), dtype=torch.uint8,

@@ -57,14 +57,24 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_get_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_bound: dict = {}  # entry points of the library, by name
+
+
 def _enqueue(entry: str, index: int, *args) -> None:
     """Calls a library entry point on the current stream of device `index`,
     that device made current for the call."""
-    if torch.cuda.current_device() == index:
-        _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+    fn = _bound.get(entry)
+    if fn is None:
+        fn = _bound[entry] = getattr(_lib.load(), entry)
+    if _get_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, entry)
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -171,8 +181,9 @@ _GROUP_SCORE = {"max": 0, "top2": 1}
 def _launch_balanced(logits, bias, topk, renormalize, groups, kept, scoring, group_score, scale,
                      load, weights_dtype, ids_dtype):
     T, E = logits.shape
-    w = torch.empty(T, topk, dtype=weights_dtype, device=logits.device)
-    ids = torch.empty(T, topk, dtype=ids_dtype, device=logits.device)
+    dev = logits.device
+    w = torch.empty(T, topk, dtype=weights_dtype, device=dev)
+    ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
     _enqueue("moe_balanced_topk", logits.get_device(), logits.data_ptr(), _code(logits),
              None if bias is None else bias.data_ptr(), T, E, topk, renormalize, groups, kept,
              group_score, scoring, scale, w.data_ptr(), _code(w), ids.data_ptr(), _code(ids),
@@ -189,6 +200,7 @@ class _BalancedTopK(torch.autograd.Function):
         w, ids = _launch_balanced(logits, bias, topk, renormalize, groups, kept, scoring,
                                   group_score, scale, load, weights_dtype, ids_dtype)
         ctx.args = (topk, renormalize, scoring, scale)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids)
         ctx.mark_non_differentiable(ids)
         return w, ids
@@ -196,15 +208,24 @@ class _BalancedTopK(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_w, _grad_ids):
+        if grad_w is None:
+            return (None,) * 12
         logits, ids = ctx.saved_tensors
         T, E = logits.shape
         grad_w = grad_w.to(torch.float32).contiguous()
-        grad = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+        grad = torch.empty_like(logits)
         topk, renormalize, scoring, scale = ctx.args
         _enqueue("moe_balanced_topk_backward", logits.get_device(), logits.data_ptr(),
                  _code(logits), ids.data_ptr(), _code(ids), grad_w.data_ptr(), T, E, topk,
                  renormalize, scoring, scale, grad.data_ptr())
         return (grad,) + (None,) * 11
+
+
+def _check_per_expert(name: str, t: torch.Tensor, dtype: torch.dtype, logits: torch.Tensor):
+    if (t.dtype != dtype or t.shape != logits.shape[1:]
+            or t.get_device() != logits.get_device()):
+        raise ValueError(f"{name} must be a {dtype} [E] = [{logits.shape[1]}] tensor on "
+                         f"{logits.device}")
 
 
 def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
@@ -239,20 +260,18 @@ def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
         raise ValueError(f"Unsupported scoring_func: {scoring_func}")
     if group_score not in _GROUP_SCORE:
         raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORE)}")
-    E = gating_output.shape[1]
-    for name, t, dtype in (("expert_bias", expert_bias, torch.float32),
-                           ("expert_load", expert_load, torch.int32)):
-        if t is not None and (t.dtype != dtype or t.shape != (E,)
-                              or t.get_device() != gating_output.get_device()):
-            raise ValueError(f"{name} must be a {dtype} [E] = [{E}] tensor on "
-                             f"{gating_output.device}")
-    if expert_load is not None and not expert_load.is_contiguous():
-        raise ValueError("expert_load must be contiguous (it is added to in place)")
-    bias = None if expert_bias is None else _contig(expert_bias.detach())
+    if expert_bias is not None:
+        _check_per_expert("expert_bias", expert_bias, torch.float32, gating_output)
+        if not expert_bias.is_contiguous():
+            expert_bias = expert_bias.contiguous()
+    if expert_load is not None:
+        _check_per_expert("expert_load", expert_load, torch.int32, gating_output)
+        if not expert_load.is_contiguous():
+            raise ValueError("expert_load must be contiguous (it is added to in place)")
     run = _launch_balanced
     if gating_output.requires_grad and torch.is_grad_enabled():
         run = _BalancedTopK.apply
-    return run(_contig(gating_output), bias, topk, int(renormalize), num_expert_group, topk_group,
+    return run(_contig(gating_output), expert_bias, topk, int(renormalize), num_expert_group, topk_group,
                _SCORING[scoring_func], _GROUP_SCORE[group_score], float(routed_scaling_factor),
                expert_load, weights_dtype, ids_dtype)
 
