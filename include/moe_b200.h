@@ -565,10 +565,10 @@ int moe_fp8_swiglu_mlp(const void* x, int64_t ld_x, int dtype, int64_t num_rows,
                        const void* addend, int64_t ld_addend, void* out, int64_t ld_out,
                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
-/* How moe_fp8_matmul runs these sizes with 16-byte aligned 16-bit output rows
- * (no GPU needed, for 148 SMs): info[0] 1 when pairs of CTAs share tiles of 256
- * tokens on the MMA's rows (0: the weights lie there), [1] columns per tile,
- * [2] CTAs that split K, [3] CTAs launched. */
+/* How moe_fp8_matmul runs these sizes (no GPU needed, for 148 SMs): info[0] 1
+ * when pairs of CTAs share tiles of 256 tokens on the MMA's rows (0: the
+ * weights lie there), [1] columns per tile, [2] CTAs that split K, [3] CTAs
+ * launched. */
 int moe_fp8_matmul_plan(int64_t num_rows, int64_t out_cols, int64_t inner, int scale_format,
                         int32_t* info);
 

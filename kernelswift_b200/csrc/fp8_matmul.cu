@@ -855,7 +855,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
 // and feeds 32 KB instead of the 48 KB of a 128 x 256 tile of its own, which
 // needs 768 cycles of shared-memory bandwidth for the MMA's 512.
 // ---------------------------------------------------------------------------
-template <bool MX>
+template <bool MX, bool VEC>
 struct PairCfg {
   static constexpr int kBN = 256;
   static constexpr int kEpiWarps = MX ? 16 : 8;
@@ -869,12 +869,19 @@ struct PairCfg {
   static constexpr int kBox = kN / 2;                  // weight rows of a CTA's TMA box
   static constexpr int kBBytes = kBN / 2 * kKB;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = MX && !VEC ? 5 : 6;
   static constexpr int kSfbChunks = kBN / 128;
   static constexpr int kSfSlots = 2, kQuads = 4;  // scale ring: slots, quads in each
   static constexpr int kQuadBytes = 512 * (1 + kSfbChunks);
   static constexpr int kRingBytes = MX ? kSfSlots * kQuads * kQuadBytes : 0;
-  static constexpr size_t kSmem = 1024 + 512 + kRingBytes + size_t(kStages) * kStageBytes;
+  // VEC: rows of the output (and the addend) in whole 16-byte vectors. Without
+  // it a warp passes 32 rows x 64 bytes at a time through a piece of shared
+  // memory, rows 17 words apart.
+  static constexpr int kRunBytes = 64, kPitchBytes = kRunBytes + 4;
+  static constexpr int kStageOut = VEC ? 0 : 32 * kPitchBytes;
+  static constexpr size_t kSmem =
+      1024 + 512 + kRingBytes + kEpiWarps * kStageOut + size_t(kStages) * kStageBytes;
+  static_assert(kSmem <= 232448, "shared memory of an SM");
   // TMEM: one accumulator and the scale slots (UE8M0), or two k-block buffers
   static constexpr int kBufs = MX ? 1 : 2;
   static constexpr int kSfCol0 = kBufs * kBN;
@@ -999,11 +1006,11 @@ __device__ __forceinline__ uint4 pack16(const float* x) {
                       pack2<T>(x[6], x[7]));
 }
 
-template <bool MX, typename TOUT>
-__global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
+template <bool MX, bool VEC, typename TOUT>
+__global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmX,
                     const __grid_constant__ CUtensorMap tmW, const MatmulParams p) {
-  using C = PairCfg<MX>;
+  using C = PairCfg<MX, VEC>;
   constexpr int STAGES = C::kStages;
   constexpr int NB = C::kBufs;
   constexpr int COLS = C::kCols;
@@ -1013,7 +1020,9 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
   uint8_t* sA = smem;
   uint8_t* sB = sA + STAGES * kABytes;
   uint8_t* sRing = sB + STAGES * C::kBBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sRing + C::kRingBytes);  // used in the even CTA
+  uint8_t* sOut = sRing + C::kRingBytes;
+  uint64_t* full =
+      reinterpret_cast<uint64_t*>(sOut + C::kEpiWarps * C::kStageOut);  // used in the even CTA
   uint64_t* empty = full + STAGES;
   uint64_t* sfull = empty + STAGES;  // used in the even CTA
   uint64_t* sempty = sfull + C::kSfSlots;
@@ -1348,37 +1357,78 @@ __global__ void __launch_bounds__(PairCfg<MX>::kThreads, 1)
         }
         if (!ok) break;
       }
-      // N is a multiple of kVec here. A quad of lanes trades vectors so that
-      // it stores 64 bytes of one row at a time (and reads the addend so).
       TOUT* out = static_cast<TOUT*>(p.out) + n0;
       const TOUT* add = static_cast<const TOUT*>(p.add) + n0;
-      const int64_t t4 = t - (lane & 3);
-      const int mine = (lane & 3) * kVec;
+      if constexpr (!VEC) {
+        // A row's 64 bytes go to memory as elements of neighbouring lanes.
+        constexpr int kRun = C::kRunBytes / int(sizeof(TOUT));
+        constexpr int kPitch = C::kPitchBytes / int(sizeof(TOUT));
+        TOUT* const piece = reinterpret_cast<TOUT*>(sOut + (warp - 4) * C::kStageOut);
+        const int64_t t32 = t - lane;
+        const int c = lane % kRun;
 #pragma unroll
-      for (int j = 0; j < COLS; j += 4 * kVec) {
-        const bool in = n0 + j + mine < p.N;
-        uint4 v[4];
-        if (p.add != nullptr) {
+        for (int j = 0; j < COLS; j += kRun) {
+          if (n0 + j >= p.N) break;
+          const bool in = n0 + j + c < p.N;
+          if (p.add != nullptr) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            v[r] = in && t4 + r < p.T
-                       ? *reinterpret_cast<const uint4*>(add + (t4 + r) * p.ld_add + j + mine)
-                       : make_uint4(0, 0, 0, 0);
+            for (int r0 = 0; r0 < 32; r0 += 32 / kRun) {
+              const int r = r0 + lane / kRun;
+              piece[r * kPitch + c] =
+                  in && t32 + r < p.T ? add[(t32 + r) * p.ld_add + j + c] : from_f32<TOUT>(0.0f);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) acc[j + k] += to_f32(piece[lane * kPitch + k]);
+          }
+          uint32_t* const words = reinterpret_cast<uint32_t*>(piece + lane * kPitch);
+#pragma unroll
+          for (int h = 0; h < C::kRunBytes / 16; ++h) {
+            const uint4 v = pack16<TOUT>(&acc[j + h * kVec]);
+            words[4 * h] = v.x;
+            words[4 * h + 1] = v.y;
+            words[4 * h + 2] = v.z;
+            words[4 * h + 3] = v.w;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 32 / kRun) {
+            const int r = r0 + lane / kRun;
+            if (in && t32 + r < p.T) out[(t32 + r) * p.ld_out + j + c] = piece[r * kPitch + c];
+          }
+          __syncwarp();
+        }
+      } else {
+        // N is a multiple of kVec. A quad of lanes trades vectors so that it
+        // stores 64 bytes of one row at a time (and reads the addend so).
+        const int64_t t4 = t - (lane & 3);
+        const int mine = (lane & 3) * kVec;
+#pragma unroll
+        for (int j = 0; j < COLS; j += 4 * kVec) {
+          const bool in = n0 + j + mine < p.N;
+          uint4 v[4];
+          if (p.add != nullptr) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              v[r] = in && t4 + r < p.T
+                         ? *reinterpret_cast<const uint4*>(add + (t4 + r) * p.ld_add + j + mine)
+                         : make_uint4(0, 0, 0, 0);
+            quad_transpose(v, lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const TOUT* e = reinterpret_cast<const TOUT*>(&v[r]);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) acc[j + r * kVec + k] += to_f32(e[k]);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = pack16<TOUT>(&acc[j + r * kVec]);
           quad_transpose(v, lane);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const TOUT* e = reinterpret_cast<const TOUT*>(&v[r]);
-#pragma unroll
-            for (int k = 0; k < kVec; ++k) acc[j + r * kVec + k] += to_f32(e[k]);
-          }
+          for (int r = 0; r < 4; ++r)
+            if (in && t4 + r < p.T)
+              *reinterpret_cast<uint4*>(out + (t4 + r) * p.ld_out + j + mine) = v[r];
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = pack16<TOUT>(&acc[j + r * kVec]);
-        quad_transpose(v, lane);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (in && t4 + r < p.T)
-            *reinterpret_cast<uint4*>(out + (t4 + r) * p.ld_out + j + mine) = v[r];
       }
     }
   }
@@ -1406,9 +1456,7 @@ struct Plan {
   int ctas;
 };
 
-// `vec`: the output's rows (and the addend's) start on 16-byte boundaries,
-// as the pair kernel's stores need.
-Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, bool vec, int sms) {
+Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
   const int64_t kbs = ceil_div(K, kKB);
   Plan best = {0, 16, 1, 1};
   double best_cost = 1e300;
@@ -1437,7 +1485,7 @@ Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, bool vec, int sms) {
       }
     }
   }
-  if (vec && T > 128) {
+  if (T > 128) {
     const int64_t tiles = ceil_div(T, 256) * ceil_div(N, 256);
     const double waves = double(ceil_div(tiles, sms / 2));
     const double cost = waves * (kbs * (mx ? 540.0 : 620.0) + (mx ? 1000 : 600)) + 1500;
@@ -1507,31 +1555,34 @@ int dispatch_cols(const Plan& plan, const CUtensorMap& w, const CUtensorMap& x,
   return fail(MOE_ERR_UNSUPPORTED, "fp8_matmul: no such tile");
 }
 
-template <bool MX, typename TOUT>
+template <bool MX, bool VEC, typename TOUT>
 int launch_pair(const Plan& plan, const CUtensorMap& w, const CUtensorMap& x,
                 const MatmulParams& p, cudaStream_t s) {
-  using C = PairCfg<MX>;
+  using C = PairCfg<MX, VEC>;
   static std::atomic<uint64_t> done{0};
-  int st = set_smem_once(fp8_pair_kernel<MX, TOUT>, C::kSmem, done);
+  int st = set_smem_once(fp8_pair_kernel<MX, VEC, TOUT>, C::kSmem, done);
   if (st != MOE_OK) return st;
   // a register split that the launch cannot cover would never return
   static const int regs = [] {
     cudaFuncAttributes attr;
-    return cudaFuncGetAttributes(&attr, fp8_pair_kernel<MX, TOUT>) == cudaSuccess ? attr.numRegs
+    return cudaFuncGetAttributes(&attr, fp8_pair_kernel<MX, VEC, TOUT>) == cudaSuccess ? attr.numRegs
                                                                                   : -1;
   }();
   KSW_REQUIRE(MX || regs == C::kLaunchRegs, MOE_ERR_UNSUPPORTED,
               "fp8_matmul: compiled register count does not match the setmaxnreg split");
-  return launch_clusters(fp8_pair_kernel<MX, TOUT>, plan.ctas, C::kThreads, C::kSmem, 2, s, x, w,
+  return launch_clusters(fp8_pair_kernel<MX, VEC, TOUT>, plan.ctas, C::kThreads, C::kSmem, 2, s, x, w,
                          p);
 }
 
 template <typename TOUT>
-int run_matmul(const Plan& plan, bool mx, const CUtensorMap& w, const CUtensorMap& x,
+int run_matmul(const Plan& plan, bool mx, bool vec, const CUtensorMap& w, const CUtensorMap& x,
                const MatmulParams& p, cudaStream_t s) {
+  if (plan.pair && vec)
+    return mx ? launch_pair<true, true, TOUT>(plan, w, x, p, s)
+              : launch_pair<false, true, TOUT>(plan, w, x, p, s);
   if (plan.pair)
-    return mx ? launch_pair<true, TOUT>(plan, w, x, p, s)
-              : launch_pair<false, TOUT>(plan, w, x, p, s);
+    return mx ? launch_pair<true, false, TOUT>(plan, w, x, p, s)
+              : launch_pair<false, false, TOUT>(plan, w, x, p, s);
   return mx ? dispatch_cols<true, TOUT>(plan, w, x, p, s)
             : dispatch_cols<false, TOUT>(plan, w, x, p, s);
 }
@@ -1557,8 +1608,7 @@ extern "C" int moe_fp8_matmul_plan(int64_t num_rows, int64_t out_cols, int64_t i
   int st = check_sizes(num_rows, out_cols, inner, scale_format);
   if (st != MOE_OK) return st;
   KSW_REQUIRE(info != nullptr, MOE_ERR_INVALID_ARG, "fp8_matmul_plan: null pointer");
-  const Plan plan =
-      plan_matmul(num_rows, out_cols, inner, scale_format == 1, out_cols % 8 == 0, 148);
+  const Plan plan = plan_matmul(num_rows, out_cols, inner, scale_format == 1, 148);
   info[0] = plan.pair;
   info[1] = plan.bn;
   info[2] = plan.splits;
@@ -1593,13 +1643,13 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   const int vec = out_dtype == MOE_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
   const bool aligned = out_cols % vec == 0 && ld_out % vec == 0 && aligned16(out) &&
                        (addend == nullptr || (ld_addend % vec == 0 && aligned16(addend)));
-  const Plan plan = plan_matmul(num_rows, out_cols, inner, mx, aligned, sms);
+  const Plan plan = plan_matmul(num_rows, out_cols, inner, mx, sms);
   CUtensorMap tx, tw;
   const uint32_t x_box = plan.pair ? kLanes : uint32_t(plan.bn);
   st = encode_tma_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, uint64_t(inner),
                      uint64_t(num_rows), uint64_t(ld_x), kKB, x_box);
   if (st != MOE_OK) return st;
-  const uint32_t w_box = plan.pair ? (mx ? PairCfg<true>::kBox : PairCfg<false>::kBox) : kLanes;
+  const uint32_t w_box = plan.pair ? (mx ? PairCfg<true, true>::kBox : PairCfg<false, true>::kBox) : kLanes;
   st = encode_tma_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, uint64_t(inner),
                      uint64_t(out_cols), uint64_t(ld_w), kKB, w_box);
   if (st != MOE_OK) return st;
@@ -1622,7 +1672,7 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   p.status = status;
   p.wait_limit_ns = kWaitLimitNs;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (out_dtype == MOE_DTYPE_F32) return run_matmul<float>(plan, mx, tw, tx, p, s);
-  if (out_dtype == MOE_DTYPE_BF16) return run_matmul<__nv_bfloat16>(plan, mx, tw, tx, p, s);
-  return run_matmul<__half>(plan, mx, tw, tx, p, s);
+  if (out_dtype == MOE_DTYPE_F32) return run_matmul<float>(plan, mx, aligned, tw, tx, p, s);
+  if (out_dtype == MOE_DTYPE_BF16) return run_matmul<__nv_bfloat16>(plan, mx, aligned, tw, tx, p, s);
+  return run_matmul<__half>(plan, mx, aligned, tw, tx, p, s);
 }

@@ -215,6 +215,22 @@ def test_large_products_by_rows(cuda_device, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_products_off_alignment(cuda_device, dtype, fmt):
+    """Output and addend rows of odd pitch, inside larger buffers."""
+    T, N, K = 1300, 2403, 520
+    assert fp8.block_matmul_plan(T, N, K, fmt)["cta_pairs"] == 1
+    x, w = operands(T, N, K, fmt, cuda_device, 9)
+    add = gen(T, N + 2, seed=5, dtype=dtype).to(cuda_device)[:, 1:-1]
+    check_product(fp8.block_matmul(*x, *w, addend=add, out_dtype=dtype), x, w, add)
+    wide = torch.full((T + 1, N + 4), 7.0, dtype=dtype, device=cuda_device)
+    out = fp8.block_matmul(*x, *w, out=wide[:-1, 3:-1])
+    assert torch.equal(out, fp8.block_matmul(*x, *w, out_dtype=dtype))
+    check_product(out, x, w)
+    assert (wide[-1] == 7).all() and (wide[:, :3] == 7).all() and (wide[:, -1] == 7).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_operand_layouts(cuda_device, fmt):
     """Row-major and padded scales, rows of a wider matrix, unaligned views,
     an output inside a larger one whose other columns stay."""
