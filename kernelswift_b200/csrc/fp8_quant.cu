@@ -88,17 +88,33 @@ __device__ __forceinline__ void load8(const Tin* p, int64_t n, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
 }
 
+// 1 / x to an ulp, for a normal result.
+__device__ __forceinline__ float rcp_ulp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // silu(g) * u with sigmoid(g) = 1 / (1 + e^-g), for negative g e^g / (1 + e^g):
 // the exponential never overflows and the divisor lies between 1 and 2, where
 // the fast reciprocal is off by an ulp. exp 2 ulp, its sum and the products half
 // an ulp each: under 6 in all.
 __device__ __forceinline__ float silu_up(float g, float u) {
   const float e = expf(-fabsf(g));
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  const float r = rcp_ulp(1.0f + e);
   return g * (g < 0.0f ? e * r : r) * u;
 }
 __device__ __forceinline__ double silu_up(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+
+// Largest of eight gated values in 64 bits, `n` of which exist. Out of line: few
+// warps come here, and its registers would cost all of them their number.
+template <typename Tin>
+__device__ __noinline__ double gated_top(const Tin* g, const Tin* u, int64_t n) {
+  double top = 0.0;
+#pragma unroll 1
+  for (int e = 0; e < 8 && e < n; ++e)
+    top = fmax(top, fabs(silu_up(double(to_f32(g[e])), double(to_f32(u[e])))));
+  return top;
+}
 
 // Two e4m3 bytes, round to nearest even; a NaN stays one, beyond 448 saturates.
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
@@ -115,17 +131,43 @@ __device__ __forceinline__ Ratio ratio_of(float amax) {
   const float up = amax < 0x1p-60f ? 0x1p100f : 1.0f;
   return {0.875f * up, amax * up * 0x1p-9f};
 }
-__device__ __forceinline__ float fp32_scale(float amax) {
-  return amax > 0.0f ? amax / 448.0f : 1.0f;
-}
-
-// a / den, correctly rounded, from y = 1 / den correctly rounded: q = a y is off
-// by an ulp at most, the residual a - q den is exact in one fma, and q + residual
-// * y then rounds to the quotient (P. Markstein's theorem, 1990). den0 is den, or
-// 0 for an infinite den, whose finite quotients are q = 0.
+// a / den: q = a y is off by two ulp at most for a y = 1 / den within an ulp; the
+// residual a - q den is exact in one fma (but for its last bit), and q + residual
+// * y rounds to the quotient, with an error of 2^-21 ulp before that rounding. A
+// quotient on the midpoint of two e4m3 values, which 32 bits hold, so comes out
+// on it. den0 is den, or 0 for an infinite den, whose finite quotients are q = 0.
 __device__ __forceinline__ float quotient(float a, float den0, float y) {
   const float q = a * y;
   return fmaf(fmaf(-q, den0, a), y, q);
+}
+__device__ __forceinline__ float fp32_scale(float amax) {
+  if (amax >= 0x1p-100f && amax < INFINITY) return quotient(amax, 448.0f, 1.0f / 448.0f);
+  return amax > 0.0f ? amax / 448.0f : 1.0f;
+}
+
+// Maxima of ITERS groups over the 16 lanes of each half-warp; lane l of a half
+// gets that of group l / (16 / ITERS). While lanes hold several groups, each
+// step hands half of them to the lane that keeps those.
+template <int ITERS>
+__device__ __forceinline__ float group_max(float (&m)[ITERS], int lane) {
+  if constexpr (ITERS == 4) {
+    const bool up = lane & 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float got = __shfl_xor_sync(0xffffffffu, up ? m[i] : m[i + 2], 8);
+      m[i] = fmaxf(up ? m[i + 2] : m[i], got);
+    }
+  }
+  if constexpr (ITERS >= 2) {
+    constexpr int o = ITERS == 4 ? 4 : 8;
+    const bool up = lane & o;
+    const float got = __shfl_xor_sync(0xffffffffu, up ? m[0] : m[1], o);
+    m[0] = fmaxf(up ? m[1] : m[0], got);
+  }
+#pragma unroll
+  for (int o = 8 / ITERS; o > 0; o >>= 1)
+    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+  return m[0];
 }
 
 // ITERS: runs of 256 columns per warp. One row's warps follow one another.
@@ -175,63 +217,75 @@ __global__ void __launch_bounds__(32 * kRowWarps)
       }
     }
   }
+  float m[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    const int64_t c = c0 + 256 * i;
-    float amax = 0.0f;
-    [[maybe_unused]] float gate[8];
+    m[i] = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (GATED) {
-        gate[e] = v[i][e];
-        v[i][e] = silu_up(v[i][e], u[i][e]);
-      }
-      amax = fmaxf(amax, fabsf(v[i][e]));
+      if constexpr (GATED) v[i][e] = silu_up(v[i][e], u[i][e]);
+      m[i] = fmaxf(m[i], fabsf(v[i][e]));
     }
+  }
+  // From here to the factors of the elements a lane works on one group of its
+  // half-warp, that of run i = my_run.
+  constexpr int kShare = 16 / ITERS;  // lanes per group
+  const float amax = group_max<ITERS>(m, lane);
+  const int my_run = (lane & 15) / kShare;
+  const int64_t col = c0 - 8 * (lane & 15) + 256 * my_run;
+  const bool writer = (lane & (kShare - 1)) == 0 && col < p.K;
+  const int64_t at = t * p.s_row + col / 128 * p.s_blk;
+  float f0, f1 = 0.0f, f2 = 0.0f;
+  if constexpr (UE8M0) {
+    uint32_t b = ue8m0_byte(amax);
+    if constexpr (GATED) {
+      // a maximum within the rounding of the 32-bit silu (under 8 ulp) of
+      // 448 * 2^k decides the scale by its 64-bit value
+      const uint32_t bits = __float_as_uint(amax);
+      const int ulps = int(bits & 0x7fffffu) - 0x600000;
+      const bool near = amax > 0.0f && amax < INFINITY && ulps >= -16 && ulps <= 16;
+      if (__any_sync(0xffffffffu, near)) {
+#pragma unroll 1
+        for (int i = 0; i < ITERS; ++i) {
+          const int64_t c = c0 + 256 * i;
+          double top = gated_top(row + c, row + p.K + c, p.K - c);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    uint32_t w[4];
-    const int64_t blk = c / 128;
-    const bool writer = (lane & 15) == 0 && c < p.K;
-    if constexpr (UE8M0) {
-      uint32_t b = ue8m0_byte(amax);
-      if constexpr (GATED) {
-        // a maximum within the rounding of the 32-bit silu (under 8 ulp) of
-        // 448 * 2^k decides the scale by its 64-bit value
-        const uint32_t bits = __float_as_uint(amax);
-        const int off = int(bits & 0x7fffffu) - 0x600000;
-        const bool near = amax > 0.0f && amax < INFINITY && off >= -16 && off <= 16;
-        if (__any_sync(0xffffffffu, near)) {
-          double m = 0.0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            m = fmax(m, fabs(silu_up(double(gate[e]), double(u[i][e]))));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (near) {
+          for (int o = 8; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (near && i == my_run) {
             const int e = int(bits >> 23);
-            const double border = ldexp(1.75, e - 127);
-            b = uint32_t(min(max(e - 8 + (m > border ? 1 : 0), 0), 254));
+            b = uint32_t(min(max(e - 8 + (top > ldexp(1.75, e - 127) ? 1 : 0), 0), 254));
           }
         }
       }
-      const float inv = ue8m0_inv_scale(b);
+    }
+    f0 = ue8m0_inv_scale(b);
+    if (writer) static_cast<uint8_t*>(p.scale)[at] = uint8_t(b);
+  } else {
+    const Ratio r = ratio_of(amax);
+    f0 = r.num;
+    f1 = amax < INFINITY ? r.den : 0.0f;
+    f2 = rcp_ulp(r.den);
+    if (writer) static_cast<float*>(p.scale)[at] = fp32_scale(amax);
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * inv, v[i][2 * e + 1] * inv);
-      if (writer) static_cast<uint8_t*>(p.scale)[t * p.s_row + blk * p.s_blk] = uint8_t(b);
+  for (int i = 0; i < ITERS; ++i) {
+    const int src = (lane & 16) + kShare * i;
+    const float x0 = __shfl_sync(0xffffffffu, f0, src);
+    uint32_t w[4];
+    if constexpr (UE8M0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * x0, v[i][2 * e + 1] * x0);
     } else {
-      const Ratio r = ratio_of(amax);
-      const float inv = 1.0f / r.den, den0 = amax < INFINITY ? r.den : 0.0f;
+      const float x1 = __shfl_sync(0xffffffffu, f1, src);
+      const float x2 = __shfl_sync(0xffffffffu, f2, src);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        w[e] = e4m3x2(quotient(v[i][2 * e] * r.num, den0, inv),
-                      quotient(v[i][2 * e + 1] * r.num, den0, inv));
-      if (writer) static_cast<float*>(p.scale)[t * p.s_row + blk * p.s_blk] = fp32_scale(amax);
+        w[e] = e4m3x2(quotient(v[i][2 * e] * x0, x1, x2), quotient(v[i][2 * e + 1] * x0, x1, x2));
     }
     // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
     // 8 bytes at a column below K are inside the row
-    if (c < p.K)
-      *reinterpret_cast<uint2*>(p.q + t * p.ld_q + c) =
+    if (c0 + 256 * i < p.K)
+      *reinterpret_cast<uint2*>(p.q + t * p.ld_q + c0 + 256 * i) =
           make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
   }
 }
