@@ -94,14 +94,37 @@ __device__ __forceinline__ float rcp_ulp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations per instruction, each rounded as by itself.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // silu(g) * u with sigmoid(g) = 1 / (1 + e^-g), for negative g e^g / (1 + e^g):
 // the exponential never overflows and the divisor lies between 1 and 2, where
 // the fast reciprocal is off by an ulp. exp 2 ulp, its sum and the products half
 // an ulp each: under 6 in all.
-__device__ __forceinline__ float silu_up(float g, float u) {
-  const float e = expf(-fabsf(g));
-  const float r = rcp_ulp(1.0f + e);
-  return g * (g < 0.0f ? e * r : r) * u;
+__device__ __forceinline__ float2 silu_up(float2 g, float2 u) {
+  const float2 e = make_float2(expf(-fabsf(g.x)), expf(-fabsf(g.y)));
+  const float2 r = make_float2(rcp_ulp(1.0f + e.x), rcp_ulp(1.0f + e.y));
+  const float2 n = mul2(e, r);
+  const float2 s = make_float2(g.x < 0.0f ? n.x : r.x, g.y < 0.0f ? n.y : r.y);
+  return mul2(mul2(g, s), u);
 }
 __device__ __forceinline__ double silu_up(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 
@@ -135,13 +158,13 @@ __device__ __forceinline__ Ratio ratio_of(float amax) {
 // residual a - q den is exact in one fma (but for its last bit), and q + residual
 // * y rounds to the quotient, with an error of 2^-21 ulp before that rounding. A
 // quotient on the midpoint of two e4m3 values, which 32 bits hold, so comes out
-// on it. den0 is den, or 0 for an infinite den, whose finite quotients are q = 0.
-__device__ __forceinline__ float quotient(float a, float den0, float y) {
-  const float q = a * y;
-  return fmaf(fmaf(-q, den0, a), y, q);
+// on it. minus is -den, or 0 for an infinite den, whose finite quotients are q = 0.
+__device__ __forceinline__ float2 quotient(float2 a, float minus, float y) {
+  const float2 q = mul2(a, both(y));
+  return fma2(fma2(q, both(minus), a), both(y), q);
 }
 __device__ __forceinline__ float fp32_scale(float amax) {
-  if (amax >= 0x1p-100f && amax < INFINITY) return quotient(amax, 448.0f, 1.0f / 448.0f);
+  if (amax >= 0x1p-100f && amax < INFINITY) return quotient(both(amax), -448.0f, 1.0f / 448.0f).x;
   return amax > 0.0f ? amax / 448.0f : 1.0f;
 }
 
@@ -222,9 +245,14 @@ __global__ void __launch_bounds__(32 * kRowWarps)
   for (int i = 0; i < ITERS; ++i) {
     m[i] = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (GATED) v[i][e] = silu_up(v[i][e], u[i][e]);
-      m[i] = fmaxf(m[i], fabsf(v[i][e]));
+    for (int e = 0; e < 8; e += 2) {
+      if constexpr (GATED) {
+        const float2 s = silu_up(make_float2(v[i][e], v[i][e + 1]),
+                                 make_float2(u[i][e], u[i][e + 1]));
+        v[i][e] = s.x;
+        v[i][e + 1] = s.y;
+      }
+      m[i] = fmaxf(m[i], fmaxf(fabsf(v[i][e]), fabsf(v[i][e + 1])));
     }
   }
   // From here to the factors of the elements a lane works on one group of its
@@ -263,7 +291,7 @@ __global__ void __launch_bounds__(32 * kRowWarps)
   } else {
     const Ratio r = ratio_of(amax);
     f0 = r.num;
-    f1 = amax < INFINITY ? r.den : 0.0f;
+    f1 = amax < INFINITY ? -r.den : 0.0f;
     f2 = rcp_ulp(r.den);
     if (writer) static_cast<float*>(p.scale)[at] = fp32_scale(amax);
   }
@@ -271,16 +299,14 @@ __global__ void __launch_bounds__(32 * kRowWarps)
   for (int i = 0; i < ITERS; ++i) {
     const int src = (lane & 16) + kShare * i;
     const float x0 = __shfl_sync(0xffffffffu, f0, src);
+    const float x1 = UE8M0 ? 0.0f : __shfl_sync(0xffffffffu, f1, src);
+    const float x2 = UE8M0 ? 0.0f : __shfl_sync(0xffffffffu, f2, src);
     uint32_t w[4];
-    if constexpr (UE8M0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = e4m3x2(v[i][2 * e] * x0, v[i][2 * e + 1] * x0);
-    } else {
-      const float x1 = __shfl_sync(0xffffffffu, f1, src);
-      const float x2 = __shfl_sync(0xffffffffu, f2, src);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = e4m3x2(quotient(v[i][2 * e] * x0, x1, x2), quotient(v[i][2 * e + 1] * x0, x1, x2));
+    for (int e = 0; e < 4; ++e) {
+      float2 a = mul2(make_float2(v[i][2 * e], v[i][2 * e + 1]), both(x0));
+      if constexpr (!UE8M0) a = quotient(a, x1, x2);
+      w[e] = e4m3x2(a.x, a.y);
     }
     // rows of q start on 16-byte boundaries and are padded to 16 bytes, so
     // 8 bytes at a column below K are inside the row
