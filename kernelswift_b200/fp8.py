@@ -86,6 +86,31 @@ def _addend(addend: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtyp
     return addend.data_ptr(), max(addend.stride(0), cols)
 
 
+def _check_apart(out: torch.Tensor, addend: torch.Tensor) -> None:
+    """out and addend are the same elements or share none: an element is read by
+    the thread that writes it, and only just before."""
+    size, cols, pitch = out.element_size(), out.shape[1], out.stride(0)
+    apart = (addend.data_ptr() - out.data_ptr()) // size
+    if not out.numel() or apart == 0 and out.stride() == addend.stride():
+        return
+    if apart >= (out.shape[0] - 1) * pitch + cols:
+        return
+    if -apart >= (out.shape[0] - 1) * addend.stride(0) + cols:
+        return
+    # columns of one wider matrix
+    if addend.stride(0) == pitch and cols <= apart % pitch <= pitch - cols:
+        return
+    raise ValueError("out and addend overlap without being the same elements")
+
+
+def _status_ptr(status: torch.Tensor | None, index: int) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.get_device() != index or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor on the operands' device")
+    return status.data_ptr()
+
+
 def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = False
                   ) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantises x [T, K] (f32/f16/bf16) to e4m3 with one scale per row and
@@ -157,7 +182,7 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     (UE8M0). Rows that do not start on 16-byte boundaries are copied first
     (quantize_rows and quantize_blocks pad them). addend [T, N] has out's
     dtype and may be out itself. Summed in fp32, rounded once to out_dtype
-    (bf16, f16 or f32). status: optional int32 device word (moe_read_status).
+    (bf16, f16 or f32; out's own dtype where it is given). status: optional int32 device word (moe_read_status).
     """
     index = x.get_device()
     if not index == w.get_device() == x_scale.get_device() == w_scale.get_device() or index < 0:
@@ -184,14 +209,19 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         out_dtype = out.dtype
         _check_out(out, T, N, out_dtype, index)
         ld_out = max(out.stride(0), N)
+        if addend is not None:
+            _check_apart(out, addend)
     add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, N, out_dtype, index)
+    if x_scale.requires_grad or w_scale.requires_grad:
+        _no_grad_needed("x_scale", x_scale)
+        _no_grad_needed("w_scale", w_scale)
     if not w_scale.is_contiguous():
         w_scale = w_scale.contiguous()
     pitch = (K + 15) // 16 * 16
     _enqueue("moe_fp8_matmul", index, x.data_ptr(), max(x.stride(0), pitch), x_scale.data_ptr(),
              *x_scale.stride(), w.data_ptr(), max(w.stride(0), pitch), w_scale.data_ptr(), fmt, T,
              N, K, add_ptr, add_ld, out.data_ptr(), ld_out, _FLOAT_CODE[out_dtype],
-             None if status is None else status.data_ptr())
+             _status_ptr(status, index))
     return out
 
 
@@ -228,7 +258,9 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
                         ("w2_scale", w2_scale)):
             _check_cuda(name, t)
         raise ValueError("x and the weights with their scales must be on one device")
-    _no_grad_needed("x", x)
+    for name, t in (("x", x), ("w13_scale", w13_scale), ("w2_scale", w2_scale)):
+        if t.requires_grad:
+            _no_grad_needed(name, t)
     if x.dim() != 2 or x.dtype not in _FLOAT or x.shape[1] < 1:
         raise ValueError("x must be a 2-D f32/f16/bf16 tensor")
     w13, w2 = _fp8_rows("w13", w13), _fp8_rows("w2", w2)
@@ -248,6 +280,8 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     else:
         _check_out(out, T, H, x.dtype, index)
+        if addend is not None:
+            _check_apart(out, addend)
     add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, H, x.dtype, index)
     code = _DTYPE_CODE[x.dtype]
     # of its own: a workspace kept by stream would be shared by captured graphs
@@ -258,5 +292,5 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
              w13.data_ptr(), max(w13.stride(0), _round_up(H, 16)), w13_scale.data_ptr(),
              w2.data_ptr(), max(w2.stride(0), _round_up(inter, 16)), w2_scale.data_ptr(), fmt,
              add_ptr, add_ld, out.data_ptr(), max(out.stride(0), H), ws.data_ptr(), ws.numel(),
-             None if status is None else status.data_ptr())
+             _status_ptr(status, index))
     return out

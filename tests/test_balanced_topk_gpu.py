@@ -250,6 +250,52 @@ def test_captured_and_on_another_stream(cuda_device):
         check(logits, bias, w, ids, k, num_expert_group=8, topk_group=4)
 
 
+@pytest.mark.parametrize("score,renorm", [("sigmoid", True), ("softmax", False)])
+def test_captured_training_step(cuda_device, score, renorm):
+    T, E, k = 70, 64, 6
+    logits, bias = inputs(T, E, torch.float32, 3)
+    b = bias.to(cuda_device)
+    x = torch.zeros(T, E, device=cuda_device, requires_grad=True)
+    gw = torch.randn(T, k, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    load = torch.zeros(E, dtype=torch.int32, device=cuda_device)
+
+    def step():
+        w, ids = fm.balanced_topk(x, x, b, k, renormalize=renorm, scoring_func=score,
+                                  expert_load=load)
+        return w, ids, *torch.autograd.grad(w, x, gw)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    with torch.no_grad():
+        x.copy_(logits)
+    graph.replay()
+    graph.replay()
+    counts, _ = load.clone(), load.zero_()
+    eager = step()
+    for g, e in zip(captured, eager):
+        assert torch.equal(g, e)
+    assert torch.equal(counts, 2 * load)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    E, k = 1024, 8
+    T = 2 ** 31 // E + 700
+    x = torch.zeros(T, E, dtype=torch.bfloat16, device=cuda_device)
+    logits, bias = inputs(3, E, torch.bfloat16, 8)
+    rows = torch.tensor([5, T - 2, T - 1], device=cuda_device)
+    x[rows] = logits.to(cuda_device)
+    x.requires_grad_()
+    w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k)
+    check(logits, bias, w[rows], ids[rows], k)
+    grad, = torch.autograd.grad(w[rows[1:]].sum() * 2 + w[rows[:1], 0].sum(), x)
+    small = logits.to(cuda_device).requires_grad_()
+    w, _ = fm.balanced_topk(small, small, bias.to(cuda_device), k)
+    want, = torch.autograd.grad(w[1:].sum() * 2 + w[:1, 0].sum(), small)
+    assert torch.equal(grad[rows], want)
+    assert not grad[6:T - 2].any()
+
+
 def test_refusals(cuda_device):
     from kernelswift_b200._lib import MoeError
 

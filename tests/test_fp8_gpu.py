@@ -1,5 +1,9 @@
 """GPU: the dense block-scaled fp8 operators (quantize_rows, quantize_blocks,
 block_matmul, swiglu_mlp) against their fp64 restatement in the oracle."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -8,6 +12,7 @@ from kernelswift_b200 import fused_moe as fm
 from oracle import moe_oracle as orc
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parents[1]
 
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -267,6 +272,96 @@ def test_nan_and_inf_stay_in_their_rows(cuda_device, T, fmt):
     assert torch.equal(a[keep], b[keep]) and b[T // 2].isnan().all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_offsets_past_32_bits(cuda_device, fmt):
+    """Rows far behind the first: inputs and outputs of more than 2^32 bytes and
+    2^31 elements."""
+    K, N = 100, 40000
+    T = 2 ** 31 // N + 500
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device=cuda_device)
+    rows = torch.tensor([0, T // 2, T - 2, T - 1], device=cuda_device)
+    x[rows] = gen(4, K, dtype=torch.bfloat16).to(cuda_device)
+    w = fp8.quantize_blocks(gen(N, K, seed=1).to(cuda_device) / 10, fmt)
+    q, scale = fp8.quantize_rows(x, fmt)
+    out = fp8.block_matmul(q, scale, *w)
+    alone = fp8.quantize_rows(x[rows], fmt)
+    check_product(out[rows], alone, w)
+    assert not out[T // 2 + 1:T - 2].any()
+    del out
+    big, two = fp8.quantize_rows(x.expand(2, T, K).reshape(2 * T, K), fmt)
+    assert torch.equal(big.view(torch.uint8)[rows + T], alone[0].view(torch.uint8))
+    assert torch.equal(two[rows + T], alone[1])
+
+
+def test_long_quantised_rows(cuda_device):
+    """One call over more than 2^32 elements."""
+    T, K = 66000, 65600
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device=cuda_device)
+    x[-1] = gen(K, dtype=torch.bfloat16).to(cuda_device)
+    q, scale = fp8.quantize_rows(x)
+    one, s1 = fp8.quantize_rows(x[-1:])
+    assert torch.equal(q.view(torch.uint8)[-1:], one.view(torch.uint8))
+    assert torch.equal(scale[-1:], s1)
+    assert not q[-2].view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("T,N,K", [(100003, 8, 64), (1, 128, 100000), (2, 100001, 32),
+                                   (7, 300, 40001)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_lopsided_products(cuda_device, T, N, K, fmt):
+    x, w = operands(T, N, K, fmt, cuda_device, 4)
+    rows = torch.arange(0, T, max(1, T // 40), device=cuda_device)
+    xq = x[0].view(torch.uint8)[rows].view(torch.float8_e4m3fn)
+    check_product(fp8.block_matmul(*x, *w, out_dtype=torch.float32)[rows], (xq, x[1][rows]), w)
+
+
+def test_first_calls_of_a_process_captured(cuda_device):
+    """Nothing has to run eagerly before a capture."""
+    code = """
+import torch
+from kernelswift_b200 import fp8, fused_moe as fm
+dev = torch.device("cuda", 0)
+x = torch.randn(300, 640, device=dev).bfloat16()
+logits = torch.randn(300, 64, device=dev)
+def layer(fmt):
+    w13 = fp8.quantize_blocks(a, fmt)
+    w2 = fp8.quantize_blocks(b, fmt)
+    return fp8.swiglu_mlp(x, *w13, *w2), fm.balanced_topk(x, logits, None, 4)[0]
+a = torch.randn(768, 640, device=dev) / 25
+b = torch.randn(640, 384, device=dev) / 20
+for fmt in ("fp32", "ue8m0"):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(fmt)
+    graph.replay()
+    want = layer(fmt)
+    assert all(torch.equal(g, w) for g, w in zip(got, want)), fmt
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True,
+                          timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls on two streams share nothing."""
+    work = []
+    for seed in range(2):
+        x = gen(500, 640, seed=seed, dtype=torch.bfloat16).to(cuda_device)
+        w13 = fp8.quantize_blocks(gen(768, 640, seed=2 + seed).to(cuda_device) / 25)
+        w2 = fp8.quantize_blocks(gen(640, 384, seed=4 + seed).to(cuda_device) / 20)
+        work.append((x, *w13, *w2))
+    want = [fp8.swiglu_mlp(*w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(20):
+        got = []
+        for w, s in zip(work, streams):
+            with torch.cuda.stream(s):
+                got.append(fp8.swiglu_mlp(*w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
 def test_no_rows_and_zero_scales(cuda_device):
     x, w = operands(4, 64, 256, "fp32", cuda_device)
     out = fp8.block_matmul(x[0][:0], x[1][:0], *w)
@@ -373,9 +468,21 @@ def test_layer_of_routed_and_shared_experts(cuda_device):
     assert orc.rel_l2(out.double().cpu(), want) < 8e-2
 
 
+def test_addend_beside_the_output(cuda_device):
+    """Columns of one buffer that share no element with the output."""
+    x, w = operands(40, 64, 256, "ue8m0", cuda_device)
+    wide = gen(40, 200, dtype=torch.bfloat16).to(cuda_device)
+    for at, to in ((100, 3), (0, 64), (64, 0)):
+        buf = wide.clone()
+        want = fp8.block_matmul(*x, *w, addend=wide[:, at:at + 64].contiguous())
+        fp8.block_matmul(*x, *w, addend=buf[:, at:at + 64], out=buf[:, to:to + 64])
+        assert torch.equal(buf[:, to:to + 64], want)
+
+
 def test_refusals(cuda_device):
     x, w = operands(4, 64, 256, "fp32", cuda_device)
     xu, wu = operands(4, 64, 256, "ue8m0", cuda_device)
+    both = torch.zeros(5, 65, dtype=torch.bfloat16, device=cuda_device)
     bad = [
         lambda: fp8.block_matmul(x[0], x[1], w[0], wu[1]),            # mixed formats
         lambda: fp8.block_matmul(x[0], x[1][:3], *w),
@@ -393,6 +500,13 @@ def test_refusals(cuda_device):
         lambda: fp8.quantize_rows(torch.zeros(4, 4, device=cuda_device, requires_grad=True)),
         lambda: fp8.quantize_blocks(torch.zeros(4, 4, device=cuda_device).int()),
         lambda: fp8.swiglu_mlp(torch.zeros(4, 256, device=cuda_device), *w, *w),
+        lambda: fp8.block_matmul(*x, *w, status=torch.zeros(1, dtype=torch.int32)),
+        lambda: fp8.block_matmul(*x, *w, status=torch.zeros(1, device=cuda_device)),
+        lambda: fp8.block_matmul(x[0], x[1].clone().requires_grad_(), *w),
+        lambda: fp8.block_matmul(*x, *w, addend=torch.zeros(1, 64, device=cuda_device,
+                                                            dtype=torch.bfloat16).expand(4, 64)),
+        lambda: fp8.block_matmul(*x, *w, out=both[:4, :64], addend=both[:4, 1:]),
+        lambda: fp8.block_matmul(*x, *w, out=both[:4, :64], addend=both[1:, :64]),
     ]
     for call in bad:
         with pytest.raises(ValueError):
