@@ -1456,40 +1456,57 @@ struct Plan {
   int ctas;
 };
 
+// Nanoseconds by a model whose constants were fitted to the measured times of
+// every plan at 51 products (T 1 to 4096, N 512 to 36864, K 300 to 18432): the
+// tiles that an SM takes one after another, each its k-blocks and its epilogue.
+// What a k-block costs is the way through the ring (kb, kb_col) or, with two
+// CTAs on an SM, the bytes and columns of both (share, share_col). Its choice
+// was 1.02 times the best plan's time on average and 1.2 times at worst.
+struct PlanCost {
+  double kb, kb_col, share, share_col, tile, tile_col, split, split_col, pair_kb, pair_tile;
+};
+constexpr PlanCost kCost[2] = {
+    {250, 1.7, 150, 2.5, 450, 8, 1250, 20, 580, 2400},  // fp32 scales
+    {265, 0.3, 170, 0.4, 0, 15, 1100, 28, 275, 3400}};  // UE8M0
+
+// Both sides measured, UE8M0, one B200, back to back: 16 x 4096 x 7168 in 4
+// pieces 9.3 us, unsplit 17.4; 128 x 7168 x 2048 in tiles of 32 tokens 8.6 us,
+// of 128 10.0, of 128 in two pieces 12.4; 512 x 4096 x 7168 as pairs 21.8 us, in
+// tiles of 128 22.0; 1024 x 4096 x 7168 25.4 and 38.8. fp32 scales: 512 x 4096 x
+// 7168 as pairs 37.1 us, in tiles of 128 29.2; 1024 x 4096 x 7168 39.2 and 55.4.
 Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
   const int64_t kbs = ceil_div(K, kKB);
+  const PlanCost& c = kCost[mx];
   Plan best = {0, 16, 1, 1};
   double best_cost = 1e300;
   for (int bn : {16, 32, 64, 128, 256}) {
     if (bn == 256 && !mx) continue;
     if (bn > 16 && bn / 2 >= T) continue;  // the half would hold every token
     const int64_t tiles = ceil_div(T, bn) * ceil_div(N, kLanes);
-    for (int s = 1; s <= 8 && s <= kbs; ++s) {
-      // the partials that a CTA receives fit their buffer for powers of two
-      if (bn == 32 && (s & (s - 1)) != 0) continue;
-      const int occ = bn <= 64 ? 2 : 1;
-      if (s > 1 && tiles * s > int64_t(sms) * occ) break;
-      // cycles: k-blocks one after another on an SM, each the MMA's or, when
-      // longer, its share of the bytes an SM takes in (and, for fp32 scales,
-      // the promotion of its columns); then a tile's epilogue
-      double per_kb = std::max(3.0 * bn, (kABytes + bn * kKB) / 56.0);
-      if (!mx) per_kb = std::max(per_kb, 200 + 3.0 * bn);
-      const double per_tile = 400 + 4.0 * bn;
-      const double waves = double(ceil_div(tiles * s, sms));
-      const double cost = waves * (double(ceil_div(kbs, s)) * per_kb + per_tile) +
-                          (s > 1 ? 1200 + 2.0 * bn : 0);
+    const int occ = bn <= 64 ? 2 : 1;
+    // clusters of other sizes leave SMs idle: 16 x 7168 x 18432 in 4 pieces
+    // 24.3 us, in 5 28.6
+    for (int s = 1; s <= 8 && s <= kbs; s *= 2) {
+      const int64_t ctas = tiles * s;
+      if (s > 1 && ctas > int64_t(sms) * occ) break;
+      // 1 also for no tokens at all
+      const int64_t on_sm = ctas > sms ? occ : 1;
+      const double rounds = double(ceil_div(ctas, sms * on_sm));
+      const double kb =
+          std::max(c.kb + c.kb_col * bn, double(on_sm) * (c.share + c.share_col * bn));
+      const double cost = rounds * (double(ceil_div(kbs, s)) * kb + c.tile + c.tile_col * bn) +
+                          (s > 1 ? c.split + c.split_col * bn : 0);
       if (cost < best_cost) {
         best_cost = cost;
-        best = {0, bn, s,
-                int(s > 1 ? tiles * s : std::min<int64_t>(tiles, int64_t(sms) * occ))};
+        best = {0, bn, s, int(std::min<int64_t>(ctas, int64_t(sms) * occ))};
       }
     }
   }
   if (T > 128) {
     const int64_t tiles = ceil_div(T, 256) * ceil_div(N, 256);
-    const double waves = double(ceil_div(tiles, sms / 2));
-    const double cost = waves * (kbs * (mx ? 540.0 : 620.0) + (mx ? 1000 : 600)) + 1500;
-    if (cost < best_cost) best = {1, 256, 1, int(2 * std::min<int64_t>(tiles, sms / 2))};
+    const double rounds = double(ceil_div(tiles, sms / 2));
+    if (rounds * (kbs * c.pair_kb + c.pair_tile) < best_cost)
+      best = {1, 256, 1, int(2 * std::min<int64_t>(tiles, sms / 2))};
   }
   return best;
 }
