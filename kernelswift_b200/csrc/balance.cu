@@ -18,8 +18,10 @@
 //
 // One warp per token, the row in registers (lane l holds experts l, l + 32,
 // ...). Group values are reduced from shared memory by 32 / G lanes per group
-// at once. What bounds it: instruction issue and latency, not its T*E*4
-// bytes.
+// at once. What bounds it: instruction issue and latency, not its T*E*4 bytes
+// (about 1300 instructions per token of 256 experts in 8 groups). One B200: 8192
+// x 256 in 8 groups, top 8, 15.4 us; 4096 x 128 7.3 us; 16384 x 384 38 us; one token
+// of 256 3.8 us.
 #include <atomic>
 #include <type_traits>
 
@@ -28,7 +30,8 @@
 namespace ksw {
 namespace {
 
-constexpr int kMaxWarps = 4;  // warps (tokens) per block
+// Warps (tokens) per block; 1 and 2 measured the same from 1 to 16384 tokens.
+constexpr int kWarps = 4;
 
 struct BalanceParams {
   const void* logits;
@@ -396,17 +399,20 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   return sel;
 }
 
+// 64 registers for up to 256 experts: 8192 x 256 15.4 us, 16.3 with 80. The
+// parameters stay in constant memory, where the functions out of line read them
+// too (a copy in each thread's local memory cost 1.3 us there).
 template <int PL, typename Tin>
-__global__ void __launch_bounds__(32 * kMaxWarps, PL <= 8 ? 8 : 4)
-    balanced_topk_kernel(const BalanceParams p) {
+__global__ void __launch_bounds__(32 * kWarps, PL <= 8 ? 8 : 4)
+    balanced_topk_kernel(const __grid_constant__ BalanceParams p) {
   extern __shared__ double s_scratch[];
-  __shared__ int s_list[kMaxWarps][32];
+  __shared__ int s_list[kWarps][32];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int warps = blockDim.x >> 5;
   double* scratch = s_scratch + (p.G > 1 ? warp * (p.E + p.G) : 0);
-  for (int64_t t = int64_t(blockIdx.x) * warps + warp; t < p.T; t += int64_t(gridDim.x) * warps) {
+  for (int64_t t = int64_t(blockIdx.x) * kWarps + warp; t < p.T;
+       t += int64_t(gridDim.x) * kWarps) {
     const Tin* row = static_cast<const Tin*>(p.logits) + t * p.E;
     float l[PL];
     float mx = -INFINITY;
@@ -471,7 +477,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, PL <= 8 ? 8 : 4)
 //                          (p is the softmax over the chosen alone)
 //   softmax:               dl_e = s_e (g_e - sum_i g_i s_i), g_e = 0 elsewhere
 // One warp per token: it fills the row, then lane j < k stores expert j's
-// entry. Bound by the T*E*b bytes it writes (and reads, for the last form).
+// entry. Bound by the T*E*b bytes it writes (and reads, for the last form); at
+// 4096 x 128 bf16 it takes 3.2 us (4.7 us in the last form), a fraction of what the
+// autograd engine takes to call it.
 // ---------------------------------------------------------------------------
 
 struct BalanceGradParams {
@@ -486,15 +494,15 @@ struct BalanceGradParams {
 };
 
 template <typename Tin>
-__global__ void __launch_bounds__(32 * kMaxWarps)
+__global__ void __launch_bounds__(32 * kWarps)
     balanced_topk_grad_kernel(const BalanceGradParams p) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int warps = blockDim.x >> 5;
   constexpr int kVec = 16 / int(sizeof(Tin));
   const bool vec = p.E % kVec == 0;  // every row starts on a 16-byte boundary
-  for (int64_t t = int64_t(blockIdx.x) * warps + warp; t < p.T; t += int64_t(gridDim.x) * warps) {
+  for (int64_t t = int64_t(blockIdx.x) * kWarps + warp; t < p.T;
+       t += int64_t(gridDim.x) * kWarps) {
     const Tin* row = static_cast<const Tin*>(p.logits) + t * p.E;
     Tin* out = static_cast<Tin*>(p.grad_logits) + t * p.E;
     const bool mine = lane < p.k;
@@ -551,18 +559,12 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
   }
 }
 
-// One token per block while that leaves SMs free, else kMaxWarps tokens.
-int pick_warps(int64_t T) { return T <= 148 * kMaxWarps ? 1 : kMaxWarps; }
-int pick_grid(int64_t T, int warps) {
-  return int(std::min<int64_t>(ceil_div(T, warps), 148 * 64));
-}
+int grid_for(int64_t T) { return int(std::min<int64_t>(ceil_div(T, kWarps), 148 * 64)); }
 
 template <int PL, typename Tin>
 int launch_balanced(const BalanceParams& p, cudaStream_t s) {
-  const int warps = pick_warps(p.T);
-  const size_t smem = p.G > 1 ? size_t(warps) * (p.E + p.G) * sizeof(double) : 0;
-  KSW_LAUNCH(balanced_topk_kernel<PL, Tin>, dim3(pick_grid(p.T, warps)), dim3(32 * warps), smem, s,
-             p);
+  const size_t smem = p.G > 1 ? size_t(kWarps) * (p.E + p.G) * sizeof(double) : 0;
+  KSW_LAUNCH(balanced_topk_kernel<PL, Tin>, dim3(grid_for(p.T)), dim3(32 * kWarps), smem, s, p);
   return MOE_OK;
 }
 
@@ -579,9 +581,7 @@ int launch_balanced_e(const BalanceParams& p, cudaStream_t s) {
 
 template <typename Tin>
 int launch_grad(const BalanceGradParams& p, cudaStream_t s) {
-  const int warps = pick_warps(p.T);
-  KSW_LAUNCH(balanced_topk_grad_kernel<Tin>, dim3(pick_grid(p.T, warps)), dim3(32 * warps), 0, s,
-             p);
+  KSW_LAUNCH(balanced_topk_grad_kernel<Tin>, dim3(grid_for(p.T)), dim3(32 * kWarps), 0, s, p);
   return MOE_OK;
 }
 

@@ -15,11 +15,22 @@
 //   lanes). Tiles too few for the SMs are split along K over a cluster of up
 //   to 8 CTAs, whose fp32 partials are summed in rank order through
 //   distributed shared memory: one launch, no workspace, a fixed order.
+//   Bound by the stream of weights and, at a few MB of them, by the fixed cost
+//   of a launch (about 3 us of barrier, TMEM and cluster set-up, pipeline fill
+//   and the last tile's way out). One B200, back to back, UE8M0: 1 x 4096 x 7168
+//   8.5 us (3.5 TB/s), 1 x 36864 x 7168 40.5 us (6.5 TB/s), 16 x 7168 x 2048 7.4
+//   us, 128 x 4096 x 7168 13.5 us; fp32 scales 8.5, 41, 7.4 and 15.2 us.
 //
 // fp8_pair_kernel: many tokens. Two CTAs share a tile of 256 tokens (lanes) x
 //   256 weight rows (columns), each holding half of either operand; with fp32
 //   scales a thread's columns share one sw and its row one sx, a single factor
-//   per thread and k-block.
+//   per thread and k-block. Bound by the tensor core at the clock that the power
+//   limit leaves (UE8M0), or by the way of a k-block's product through tensor
+//   memory and registers (fp32 scales). One B200, back to back, UE8M0: 4096 x
+//   4096 x 7168 87 us (2760 TFLOP/s), 16384 x 4096 x 7168 374 us, 8192 x 7168 x
+//   2048 94 us; fp32 scales 122 us (1970 TFLOP/s), 498 us and 140 us. Tiles of
+//   256 x 256 take an SM's shared memory 512 cycles per k-block for the 512 of its
+//   MMAs; 128 x 256 tiles of single CTAs would take 768.
 #include <atomic>
 #include <type_traits>
 
@@ -163,7 +174,10 @@ __device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* tm, int32_t c0
                "r"(c0), "r"(c1)
                : "memory");
 }
-constexpr int kL2Ahead = 6;   // k-blocks of weights a CTA asks for ahead of the wait
+// k-blocks of weights that a CTA asks L2 for while its predecessor still runs: 1 x
+// 4096 x 7168 8.96 us without, 8.58 with 6 (about what fits in the ring), slower
+// again with 16.
+constexpr int kL2Ahead = 6;
 
 // TMA producers: two warps take the stages in turn. A turn (wait for the
 // stage, announce its bytes, issue two copies) takes a warp about 490 cycles
@@ -264,7 +278,8 @@ struct ColsCfg {
   static constexpr int kGroups = kEpiWarps / 4;       // epilogue groups of 128 lanes
   // A split tile's partials: pushed into the memory of the CTA that sums them
   // where that costs no pipeline stages (BN <= 32), else read from their own
-  // CTA's memory.
+  // CTA's memory between two cluster barriers (1 x 4096 x 7168 9.7 us read,
+  // 8.6 pushed).
   static constexpr bool kPush = BN <= 32;
   static constexpr int kRecvBytes = kPush ? 16384 : 0;
   static constexpr int kOutBytes =  // staged output, or received partials
@@ -273,7 +288,7 @@ struct ColsCfg {
   static constexpr int kStages = int(((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / kStageBytes);
   static constexpr size_t kSmem = kFixed + size_t(kStages) * kStageBytes;
   // TMEM: accumulators (UE8M0) or per-k-block buffers (fp32), then scale slots
-  static constexpr int kBufs = MX ? (BN == 256 ? 1 : 2) : (BN == 256 ? 2 : 4);
+  static constexpr int kBufs = MX ? (BN == 256 ? 1 : 2) : 4;
   static constexpr int kSfCol0 = kBufs * BN;
   static constexpr int kSfCols = 4 * (1 + kSfb);
   static constexpr int kUsed = kSfCol0 + (MX ? kSfSlots * kQuads * kSfCols : 0);
@@ -1252,7 +1267,8 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
         uint8_t* dst = sRing + slot * Q * C::kQuadBytes;
         xw.store(dst, C::kQuadBytes, lane);
 #pragma unroll
-        for (int c = 0; c < C::kSfbChunks; ++c) ww[c].store(dst + 512 * (1 + c), C::kQuadBytes, lane);
+        for (int c = 0; c < C::kSfbChunks; ++c)
+          ww[c].store(dst + 512 * (1 + c), C::kQuadBytes, lane);
         // the copies to tensor memory read it through the async proxy
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -1582,13 +1598,13 @@ int launch_pair(const Plan& plan, const CUtensorMap& w, const CUtensorMap& x,
   // a register split that the launch cannot cover would never return
   static const int regs = [] {
     cudaFuncAttributes attr;
-    return cudaFuncGetAttributes(&attr, fp8_pair_kernel<MX, VEC, TOUT>) == cudaSuccess ? attr.numRegs
-                                                                                  : -1;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, fp8_pair_kernel<MX, VEC, TOUT>);
+    return e == cudaSuccess ? attr.numRegs : -1;
   }();
   KSW_REQUIRE(MX || regs == C::kLaunchRegs, MOE_ERR_UNSUPPORTED,
               "fp8_matmul: compiled register count does not match the setmaxnreg split");
-  return launch_clusters(fp8_pair_kernel<MX, VEC, TOUT>, plan.ctas, C::kThreads, C::kSmem, 2, s, x, w,
-                         p);
+  return launch_clusters(fp8_pair_kernel<MX, VEC, TOUT>, plan.ctas, C::kThreads, C::kSmem, 2, s, x,
+                         w, p);
 }
 
 template <typename TOUT>
@@ -1666,7 +1682,8 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   st = encode_tma_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, uint64_t(inner),
                      uint64_t(num_rows), uint64_t(ld_x), kKB, x_box);
   if (st != MOE_OK) return st;
-  const uint32_t w_box = plan.pair ? (mx ? PairCfg<true, true>::kBox : PairCfg<false, true>::kBox) : kLanes;
+  const uint32_t pair_box = mx ? PairCfg<true, true>::kBox : PairCfg<false, true>::kBox;
+  const uint32_t w_box = plan.pair ? pair_box : kLanes;
   st = encode_tma_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, uint64_t(inner),
                      uint64_t(out_cols), uint64_t(ld_w), kKB, w_box);
   if (st != MOE_OK) return st;
@@ -1690,6 +1707,7 @@ extern "C" int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale,
   p.wait_limit_ns = kWaitLimitNs;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (out_dtype == MOE_DTYPE_F32) return run_matmul<float>(plan, mx, aligned, tw, tx, p, s);
-  if (out_dtype == MOE_DTYPE_BF16) return run_matmul<__nv_bfloat16>(plan, mx, aligned, tw, tx, p, s);
+  if (out_dtype == MOE_DTYPE_BF16)
+    return run_matmul<__nv_bfloat16>(plan, mx, aligned, tw, tx, p, s);
   return run_matmul<__half>(plan, mx, aligned, tw, tx, p, s);
 }

@@ -14,7 +14,10 @@
 // midpoint of two e4m3 values is recognised as such (a multiplication by a
 // rounded reciprocal falls to either side of it).
 //
-// What bounds the row kernel: HBM. A half-warp holds a group (8 columns per
+// What bounds the row kernel: HBM (one B200: 4096 x 7168 bf16 14.4 us UE8M0, 6.1
+// TB/s, and 16.9 us fp32 scales; 8192 x 8192 f32 47.8 us, 7.0 TB/s), for the gated
+// form instruction issue too (4096 x 2048 11.5 us, 3.6 TB/s); a few rows are
+// latency (1 x 7168 1.2 us). A half-warp holds a group (8 columns per
 // lane, one 16-byte load for 16-bit inputs, two where rows start off such a
 // boundary), a warp up to 1024 columns of a row with its loads in flight before
 // the first is used; neighbouring warps take neighbouring columns, so that a
@@ -383,7 +386,11 @@ int launch_rows_i(const QuantRows& p, int ue8m0, cudaStream_t s) {
 template <typename Tin, bool ALIGNED, bool GATED>
 int launch_rows(const QuantRows& p, int ue8m0, cudaStream_t s) {
   // 256 columns per warp until the SMs are full of warps, then more loads in
-  // flight per warp
+  // flight per warp and, for 16-bit inputs, maxima of four groups reduced
+  // together. One B200, bf16 x 7168 columns, UE8M0: 64 rows 1.8 us against 1.9
+  // with 1024 columns per warp, 600 rows 4.2 against 3.8, 4096 rows 20.4 against
+  // 14.4; f32 8192 x 8192 49.8 us with 256, 47.8 with 512, 47.9 with 1024; gated
+  // 4096 x 2048 13.5, 11.5, 12.7.
   constexpr int kMany = GATED || sizeof(Tin) == 4 ? 2 : 4;
   if (p.T * ceil_div(p.K, 256) <= 148 * 64)
     return launch_rows_i<Tin, ALIGNED, GATED, 1>(p, ue8m0, s);

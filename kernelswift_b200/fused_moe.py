@@ -271,9 +271,9 @@ def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     run = _launch_balanced
     if gating_output.requires_grad and torch.is_grad_enabled():
         run = _BalancedTopK.apply
-    return run(_contig(gating_output), expert_bias, topk, int(renormalize), num_expert_group, topk_group,
-               _SCORING[scoring_func], _GROUP_SCORE[group_score], float(routed_scaling_factor),
-               expert_load, weights_dtype, ids_dtype)
+    return run(_contig(gating_output), expert_bias, topk, int(renormalize), num_expert_group,
+               topk_group, _SCORING[scoring_func], _GROUP_SCORE[group_score],
+               float(routed_scaling_factor), expert_load, weights_dtype, ids_dtype)
 
 
 # ---------------------------------------------------------------------------
