@@ -16,12 +16,14 @@
 // 32-bit scores (and that is not between equal logits with equal biases,
 // a true tie) sends the warp through the same code in 64 bits.
 //
-// One warp per token, the row in registers (lane l holds experts l, l + 32,
-// ...). Group values are reduced from shared memory by 32 / G lanes per group
-// at once. What bounds it: instruction issue and latency, not its T*E*4 bytes
-// (about 1300 instructions per token of 256 experts in 8 groups). One B200: 8192
-// x 256 in 8 groups, top 8, 15.4 us; 4096 x 128 7.3 us; 16384 x 384 38 us; one token
-// of 256 3.8 us.
+// One warp per token, the row in registers (lane l holds the PL experts from l PL
+// on). Where a group is the experts of a power of two of lanes, its value is
+// reduced among them; other groups' from shared memory, by 32 / G lanes per group
+// at once (8192 x 256 in 8 groups 13.7 us the first way, 15.3 the second, with lane
+// l holding experts l, l + 32, ...). What bounds it: instruction issue and latency, not its T*E*4 bytes
+// (about 1150 instructions per token of 256 experts in 8 groups). One B200: 8192
+// x 256 in 8 groups, top 8, 13.7 us; 4096 x 128 6.9 us; 16384 x 384 35 us; one token
+// of 256 3.4 us.
 #include <atomic>
 #include <type_traits>
 
@@ -39,8 +41,10 @@ struct BalanceParams {
   int64_t T;
   int E, k, G, EG, kept;
   uint32_t eg_magic;  // ceil(2^22 / EG): e / EG = (e * eg_magic) >> 22 for e < 1024, EG <= 1024
-  int lanes_per_group;  // the largest power of two with G * lanes_per_group <= 32
-  int group_shift;      // its logarithm
+  // lanes that reduce a group's value, a power of two, and its logarithm: those
+  // that hold its experts (in_lanes), else as many as 32 lanes allow
+  int lanes_per_group, group_shift, in_lanes;
+  int vec, vec_bias;  // a lane's logits and biases may be loaded as 16-byte vectors
   int softmax, top2, renorm;
   float scale;
   void* weights;
@@ -112,22 +116,53 @@ __device__ __forceinline__ float score_ulps(int softmax, float mx) {
   return softmax ? 16.0f + 0.5f * (PL + 4) : 6.0f + 1.2f * fmaxf(-mx, 0.0f);
 }
 
-// c of the row's experts, lane l's j-th being expert l + 32 j. `mx` is the
-// row's largest logit; a NaN ranks last. `smax` returns the largest score.
+// A lane's PL values of a row of E: whole vectors where the caller says so (E is
+// then a multiple of PL), `rest` behind the row's end.
+template <int PL, typename T>
+__device__ __forceinline__ void load_lane(const T* row, int E, int lane, bool vec, float rest,
+                                          float (&v)[PL]) {
+  constexpr int kBytes = PL * int(sizeof(T));
+  if constexpr (kBytes % 16 == 0) {
+    if (vec) {
+      const uint4* at = reinterpret_cast<const uint4*>(row + lane * PL);
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 w = lane * PL < E ? __ldg(at + i) : make_uint4(0, 0, 0, 0);
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < 16 / int(sizeof(T)); ++j)
+          v[i * (16 / int(sizeof(T))) + j] = lane * PL < E ? to_f32(e[j]) : rest;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    const int e = lane * PL + j;
+    v[j] = e < E ? to_f32(row[e]) : rest;
+  }
+}
+
+// c of the row's experts, lane l's j-th being expert l PL + j, -inf behind the
+// last. `mx` is the row's largest logit; a NaN ranks last. `smax` returns the
+// largest score.
 template <typename R, int PL, typename Tin>
 __device__ __forceinline__ void biased_scores(const BalanceParams& p, const float (&l)[PL],
                                               float mx, int lane, R (&c)[PL], R& smax) {
   const R rmx = mx == -INFINITY ? R(0) : R(mx);
   float b[PL];
+  if (p.bias != nullptr) {
+    load_lane<PL>(p.bias, p.E, lane, p.vec_bias, -INFINITY, b);
+  } else {
 #pragma unroll
-  for (int j = 0; j < PL; ++j)
-    b[j] = p.bias != nullptr ? __ldg(p.bias + min(lane + 32 * j, p.E - 1)) : 0.0f;
+    for (int j = 0; j < PL; ++j) b[j] = lane * PL + j < p.E ? 0.0f : -INFINITY;
+  }
   if (p.softmax) {
     R sum = R(0);
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
       c[j] = score_exp(R(l[j]) - rmx);
-      if (lane + 32 * j < p.E) sum += c[j];
+      if (lane * PL + j < p.E) sum += c[j];
     }
     sum = warp_sum(sum);
     const bool none = mx == -INFINITY;  // no expert has a score: all 0
@@ -161,21 +196,26 @@ __device__ __forceinline__ void top_two(double v, double& a, double& b) {
 template <typename R, int PL, typename Tol>
 __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R (&c)[PL],
                                                 int lane, R* scratch, Tol tol, bool& close) {
-  // position e + group keeps lanes of different groups on different banks
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    const int e = lane + 32 * j;
-    if (e < p.E) scratch[e + group_of(p, e)] = c[j];
-  }
-  __syncwarp();
   const int per = p.lanes_per_group;
   const int g = lane >> p.group_shift, sub = lane & (per - 1);
   R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
-  if (g < p.G) {
-    const R* at = scratch + g * (p.EG + 1);
+  if (p.in_lanes) {
+#pragma unroll
+    for (int j = 0; j < PL; ++j) top_two(c[j], a, b);
+  } else {
+    // position e + group keeps lanes of different groups on different banks
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      const int e = lane * PL + j;
+      if (e < p.E) scratch[e + group_of(p, e)] = c[j];
+    }
+    __syncwarp();
+    if (g < p.G) {
+      const R* at = scratch + g * (p.EG + 1);
 #pragma unroll 4
-    for (int i = sub; i < p.EG; i += per) top_two(at[i], a, b);
+      for (int i = sub; i < p.EG; i += per) top_two(at[i], a, b);
+    }
   }
   for (int o = per >> 1; o > 0; o >>= 1) {
     const R oa = __shfl_xor_sync(0xffffffffu, a, o);
@@ -199,8 +239,20 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
   close = mine && !keep && value >= last - tol(last) && last > R(-INFINITY);
   return __ballot_sync(0xffffffffu, keep);
 }
-__device__ __forceinline__ bool is_kept(const BalanceParams& p, uint32_t kept, int e) {
-  return p.G == 1 || ((kept >> (group_of(p, e) << p.group_shift)) & 1u);
+// Bit j: this lane's expert j exists and its group is kept.
+template <int PL>
+__device__ __forceinline__ uint32_t open_experts(const BalanceParams& p, uint32_t kept, int lane) {
+  const int first = lane * PL;
+  uint32_t open = first + PL <= p.E ? 0xffffffffu : first < p.E ? (1u << (p.E - first)) - 1 : 0u;
+  if (p.in_lanes) {
+    if (!((kept >> (lane & ~(p.lanes_per_group - 1))) & 1u)) open = 0;
+  } else if (p.G > 1) {
+#pragma unroll
+    for (int j = 0; j < PL; ++j)
+      if (!((kept >> (group_of(p, min(first + j, p.E - 1)) << p.group_shift)) & 1u))
+        open &= ~(1u << j);
+  }
+  return open;
 }
 
 // Puts n <= 32 candidates (lane i < n: expert `e`) in their order in 64 bits and
@@ -240,14 +292,12 @@ template <int PL, typename Tin>
 __device__ __forceinline__ void exact_scores(const BalanceParams& p, const Tin* row, float mx,
                                              int lane, double (&c)[PL]) {
   float l[PL];
-#pragma unroll
-  for (int j = 0; j < PL; ++j)
-    l[j] = lane + 32 * j < p.E ? to_f32(row[lane + 32 * j]) : -INFINITY;
+  load_lane<PL>(row, p.E, lane, p.vec, -INFINITY, l);
   double smax;
   biased_scores<double, PL, Tin>(p, l, mx, lane, c, smax);
 }
 
-// The groups kept, in 64 bits (is_kept's mask).
+// The groups kept, in 64 bits (kept_groups' mask).
 template <int PL, typename Tin>
 __device__ __noinline__ uint32_t kept_exact(const BalanceParams& p, const Tin* row, float mx,
                                             int lane, double* scratch) {
@@ -266,12 +316,7 @@ __device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row,
   uint32_t kept = 0xffffffffu;
   bool close = false;
   if (p.G > 1) kept = kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
-  uint32_t open = 0;  // bit j: expert lane + 32 j may still be chosen
-#pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    const int e = lane + 32 * j;
-    if (e < p.E && is_kept(p, kept, e)) open |= 1u << j;
-  }
+  uint32_t open = open_experts<PL>(p, kept, lane);
   int sel = 0;
   for (int s = 0; s < p.k; ++s) {
     double v = -INFINITY;
@@ -280,7 +325,7 @@ __device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row,
     for (int j = 0; j < PL; ++j)
       if (((open >> j) & 1u) && (i == INT32_MAX || c[j] > v)) {
         v = c[j];
-        i = lane + 32 * j;
+        i = lane * PL + j;
       }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -291,7 +336,7 @@ __device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row,
         i = oi;
       }
     }
-    if ((i & 31) == lane) open &= ~(1u << (i >> 5));
+    if (i / PL == lane) open &= ~(1u << (i % PL));
     if (lane == s) sel = i;
   }
   return sel;
@@ -309,8 +354,8 @@ __device__ __forceinline__ bool true_tie(const BalanceParams& p, const Tin* row,
 // those within the tolerance of the last one. The values are held as ordered
 // unsigned keys whose low bits give way to the lane's index of the expert (PL - 1
 // - j, so that ties go to the lower one), 0 for one that cannot be chosen. Each
-// lane sorts its keys; a pick is the warp-wide maximum of the lanes' first keys,
-// popped in its lane.
+// lane sorts its keys; a pick is the largest of the lanes' first keys, their low
+// bits apart, popped in the lowest lane that has it.
 template <int PL, typename Tin>
 __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row,
                                           const float (&l)[PL], float mx, int lane,
@@ -332,12 +377,10 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   }
   constexpr uint32_t kLow = PL - 1;
   uint32_t key[PL];
+  const uint32_t open = open_experts<PL>(p, kept, lane);
 #pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    const int e = lane + 32 * j;
-    const bool in = e < p.E && is_kept(p, kept, e);
-    key[j] = in ? (order_key(c[j]) & ~kLow) | (kLow - j) : 0u;
-  }
+  for (int j = 0; j < PL; ++j)
+    key[j] = (open >> j) & 1u ? (order_key(c[j]) & ~kLow) | (kLow - j) : 0u;
   // bitonic sort, descending
 #pragma unroll
   for (int w = 2; w <= PL; w <<= 1)
@@ -355,13 +398,14 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   float last = 0.0f;
   bool close = false;
   for (int s = 0; s < p.k; ++s) {
-    const uint32_t best = redux_max(key[0]);
-    const int src = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-    const int i = src + 32 * int(kLow - (best & kLow));
+    const uint32_t top = key[0] & ~kLow;
+    const uint32_t best = redux_max(top);
+    const int src = __ffs(__ballot_sync(0xffffffffu, top == best)) - 1;
+    const int i = src * PL + int(kLow - (__shfl_sync(0xffffffffu, key[0], src) & kLow));
     if (lane == s) sel = i;
 #pragma unroll
     for (int j = 0; j < PL; ++j) key[j] = lane != src ? key[j] : j + 1 < PL ? key[j + 1] : 0u;
-    const float v = key_value(best & ~kLow);
+    const float v = key_value(best);
     if (s > 0 && last - v <= tol(last) && !true_tie(p, row, last_i, i)) close = true;
     last = v;
     last_i = i;
@@ -374,7 +418,7 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
 #pragma unroll
       for (int j = 0; j < PL; ++j)
         near |= key[j] >= bar && key[j] != 0u &&
-                !true_tie(p, row, last_i, lane + 32 * int(kLow - (key[j] & kLow)));
+                !true_tie(p, row, last_i, lane * PL + int(kLow - (key[j] & kLow)));
     }
     if (__any_sync(0xffffffffu, near) || close) {
       int n = p.k;
@@ -384,7 +428,7 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
         const bool in = key[j] >= bar && key[j] != 0u;
         const uint32_t who = __ballot_sync(0xffffffffu, in);
         const int at = n + __popc(who & lanemask_lt());
-        if (in && at < 32) list[at] = lane + 32 * int(kLow - (key[j] & kLow));
+        if (in && at < 32) list[at] = lane * PL + int(kLow - (key[j] & kLow));
         n += __popc(who);
       }
       __syncwarp();
@@ -399,7 +443,7 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   return sel;
 }
 
-// 64 registers for up to 256 experts: 8192 x 256 15.4 us, 16.3 with 80. The
+// 64 registers for up to 256 experts (8192 x 256 15.4 us against 16.3 with 80). The
 // parameters stay in constant memory, where the functions out of line read them
 // too (a copy in each thread's local memory cost 1.3 us there).
 template <int PL, typename Tin>
@@ -410,18 +454,15 @@ __global__ void __launch_bounds__(32 * kWarps, PL <= 8 ? 8 : 4)
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double* scratch = s_scratch + (p.G > 1 ? warp * (p.E + p.G) : 0);
+  double* scratch = s_scratch + (p.G > 1 && !p.in_lanes ? warp * (p.E + p.G) : 0);
   for (int64_t t = int64_t(blockIdx.x) * kWarps + warp; t < p.T;
        t += int64_t(gridDim.x) * kWarps) {
     const Tin* row = static_cast<const Tin*>(p.logits) + t * p.E;
     float l[PL];
+    load_lane<PL>(row, p.E, lane, p.vec, -INFINITY, l);
     float mx = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int e = lane + 32 * j;
-      l[j] = e < p.E ? to_f32(row[e]) : -INFINITY;
-      mx = fmaxf(mx, l[j]);
-    }
+    for (int j = 0; j < PL; ++j) mx = fmaxf(mx, l[j]);
     mx = warp_max(mx);
     const int sel = select_row<PL>(p, row, l, mx, lane, scratch, s_list[warp]);
 
@@ -562,8 +603,17 @@ __global__ void __launch_bounds__(32 * kWarps)
 int grid_for(int64_t T) { return int(std::min<int64_t>(ceil_div(T, kWarps), 148 * 64)); }
 
 template <int PL, typename Tin>
-int launch_balanced(const BalanceParams& p, cudaStream_t s) {
-  const size_t smem = p.G > 1 ? size_t(kWarps) * (p.E + p.G) * sizeof(double) : 0;
+int launch_balanced(BalanceParams p, cudaStream_t s) {
+  const int held = p.EG % PL == 0 ? p.EG / PL : 0;  // lanes that hold a group
+  p.in_lanes = p.G > 1 && held > 0 && (held & (held - 1)) == 0;
+  p.lanes_per_group = 32;
+  while (p.in_lanes ? p.lanes_per_group > held : p.G * p.lanes_per_group > 32)
+    p.lanes_per_group /= 2;
+  p.group_shift = 0;
+  while ((1 << p.group_shift) < p.lanes_per_group) ++p.group_shift;
+  p.vec = p.E % PL == 0 && (p.E * sizeof(Tin)) % 16 == 0 && aligned16(p.logits);
+  p.vec_bias = p.E % PL == 0 && aligned16(p.bias);
+  const size_t smem = p.G > 1 && !p.in_lanes ? size_t(kWarps) * (p.E + p.G) * sizeof(double) : 0;
   KSW_LAUNCH(balanced_topk_kernel<PL, Tin>, dim3(grid_for(p.T)), dim3(32 * kWarps), smem, s, p);
   return MOE_OK;
 }
@@ -642,9 +692,6 @@ extern "C" int moe_balanced_topk(const void* router_logits, int logits_dtype,
   p.EG = num_experts / num_expert_group;
   p.kept = topk_group;
   p.eg_magic = uint32_t(((1 << 22) + p.EG - 1) / p.EG);
-  p.group_shift = 5;
-  while ((p.G << p.group_shift) > 32) --p.group_shift;
-  p.lanes_per_group = 1 << p.group_shift;
   p.softmax = scoring_func == 0;
   p.top2 = group_score;
   p.renorm = renormalize;
