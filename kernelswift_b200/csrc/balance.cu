@@ -20,10 +20,10 @@
 // on). Where a group is the experts of a power of two of lanes, its value is
 // reduced among them; other groups' from shared memory, by 32 / G lanes per group
 // at once (8192 x 256 in 8 groups 13.7 us the first way, 15.3 the second, with lane
-// l holding experts l, l + 32, ...). What bounds it: instruction issue and latency, not its T*E*4 bytes
-// (about 1150 instructions per token of 256 experts in 8 groups). One B200: 8192
-// x 256 in 8 groups, top 8, 13.7 us; 4096 x 128 6.9 us; 16384 x 384 35 us; one token
-// of 256 3.4 us.
+// l holding experts l, l + 32, ...). What bounds it: instruction issue and
+// latency, not its T*E*4 bytes (about 1150 instructions per token of 256 experts
+// in 8 groups). One B200: 8192 x 256 in 8 groups, top 8, 13.7 us; 4096 x 128 6.9
+// us; 16384 x 384 35 us; one token of 256 3.4 us.
 #include <atomic>
 #include <type_traits>
 

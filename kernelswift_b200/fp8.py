@@ -182,7 +182,8 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     (UE8M0). Rows that do not start on 16-byte boundaries are copied first
     (quantize_rows and quantize_blocks pad them). addend [T, N] has out's
     dtype and may be out itself. Summed in fp32, rounded once to out_dtype
-    (bf16, f16 or f32; out's own dtype where it is given). status: optional int32 device word (moe_read_status).
+    (bf16, f16 or f32; out's own dtype where it is given). status: optional
+    int32 device word (moe_read_status).
     """
     index = x.get_device()
     if not index == w.get_device() == x_scale.get_device() == w_scale.get_device() or index < 0:
