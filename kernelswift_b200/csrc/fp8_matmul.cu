@@ -179,6 +179,11 @@ __device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* tm, int32_t c0
 // again with 16.
 constexpr int kL2Ahead = 6;
 
+// Asks L2 for the line at `p`.
+__device__ __forceinline__ void l2_prefetch(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory");
+}
+
 // TMA producers: two warps take the stages in turn. A turn (wait for the
 // stage, announce its bytes, issue two copies) takes a warp about 490 cycles
 // whatever the boxes' size (570 from a single diverged lane), and a stage's
@@ -402,11 +407,20 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     const bool in = n0 + row < p.N;
     TOUT* out = static_cast<TOUT*>(p.out) + t0 * p.ld_out + n0;
     if (p.add != nullptr) {
-      const TOUT* add = static_cast<const TOUT*>(p.add) + t0 * p.ld_add + n0 + row;
+      // past the last token or column the last one again, so that the loads are
+      // unconditional and go out together
+      const TOUT* add = static_cast<const TOUT*>(p.add) + min(t0, p.T - 1) * p.ld_add +
+                        min(n0 + row, p.N - 1);
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) {
-        if (in && j < live) acc[j] += to_f32(*add);
-        add += p.ld_add;
+      for (int c = 0; c < COLS; c += 16) {
+        TOUT a[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          a[j] = *add;
+          add += c + j + 1 < live ? p.ld_add : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[c + j] += to_f32(a[j]);
       }
     }
     if (!vec) {
@@ -692,6 +706,17 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     }
     for (int i = first; epi_ok && i < tiles; i += step) {
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
+      if (p.add != nullptr) {
+        // the tile's addend is in L2 by the time its sums are done: a lane asks for
+        // the warp's 32 columns of a token
+        const int64_t n = int64_t(tile.n) * kLanes + (warp & 3) * 32;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          const int64_t t = int64_t(tile.t) * BN + col0 + c + lane;
+          if (c + lane < COLS && t < p.T && n < p.N)
+            l2_prefetch(static_cast<const TOUT*>(p.add) + t * p.ld_add + n);
+        }
+      }
       if constexpr (MX) {
         epi_ok = group_ok(1 + group, mbar_wait_bounded(&tfull[buf], bphase, abort_flag, limit));
         if (!epi_ok) break;
@@ -800,6 +825,14 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
     const int ts = p.slice, j0 = part * ts;
     const int64_t t0 = int64_t(tile.t) * BN + j0;
     if (warp >= 4 && j0 < BN && t0 < p.T) {
+      // four tokens of the addend at a time, ahead of the sums they go to
+      const TOUT* add = static_cast<const TOUT*>(p.add) + min(n, p.N - 1);
+      TOUT a[4];
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = add[min(t0 + j + e, p.T - 1) * p.ld_add];
+      };
+      if (p.add != nullptr) fetch(0);
       bool ok = mbar_wait_bounded(recv_bar, 0, abort_flag, limit);
       if (all_ok(ok) && !*abort_flag && n < p.N) {
         const float4* src = reinterpret_cast<const float4*>(sOut) + (threadIdx.x & 127) * (ts / 4);
@@ -809,16 +842,17 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
             const float4 v = src[r * kLanes * (ts / 4) + j / 4];
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
           }
-          const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+          float out[4] = {sum.x, sum.y, sum.z, sum.w};
+          if (p.add != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] += to_f32(a[e]);
+            if (j + 4 < ts) fetch(j + 4);
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int64_t t = t0 + j + e;
-            if (j0 + j + e < BN && t < p.T) {
-              float v = out[e];
-              if (p.add != nullptr)
-                v += to_f32(static_cast<const TOUT*>(p.add)[t * p.ld_add + n]);
-              static_cast<TOUT*>(p.out)[t * p.ld_out + n] = from_f32<TOUT>(v);
-            }
+            if (j0 + j + e < BN && t < p.T)
+              static_cast<TOUT*>(p.out)[t * p.ld_out + n] = from_f32<TOUT>(out[e]);
           }
         }
       }
@@ -838,6 +872,9 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
            j += int(blockDim.x >> 7) * p.splits) {
         const int64_t t = int64_t(tile.t) * BN + j;
         if (t >= p.T) break;
+        float a = 0.0f;
+        if (p.add != nullptr)
+          a = to_f32(static_cast<const TOUT*>(p.add)[t * p.ld_add + min(n, p.N - 1)]);
         float v[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r)
@@ -845,11 +882,8 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
         float sum = v[0];
 #pragma unroll
         for (int r = 1; r < 8; ++r) sum += v[r];
-        if (n < p.N) {
-          if (p.add != nullptr)
-            sum += to_f32(static_cast<const TOUT*>(p.add)[t * p.ld_add + n]);
-          static_cast<TOUT*>(p.out)[t * p.ld_out + n] = from_f32<TOUT>(sum);
-        }
+        if (p.add != nullptr) sum += a;
+        if (n < p.N) static_cast<TOUT*>(p.out)[t * p.ld_out + n] = from_f32<TOUT>(sum);
       }
     }
     cluster_sync();  // no CTA leaves while another reads its partial
@@ -1302,6 +1336,13 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
       const Tile tile = tile_at(i, p.t_tiles, p.n_tiles);
       const int64_t t = int64_t(tile.t) * 256 + rank * kLanes + row;
       const int64_t n0 = int64_t(tile.n) * C::kBN + col0;
+      if (p.add != nullptr && t < p.T) {
+        // this row's addend is in L2 by the time its sums are done
+        const TOUT* add = static_cast<const TOUT*>(p.add) + t * p.ld_add + n0;
+#pragma unroll
+        for (int j = 0; j < COLS; j += 128 / int(sizeof(TOUT)))
+          if (n0 + j < p.N) l2_prefetch(add + j);
+      }
       float acc[COLS];
       if constexpr (MX) {
         ok = mbar_wait_bounded(&my_tfull[buf], bphase, abort_flag, limit);
