@@ -18,8 +18,8 @@
 //   Bound by the stream of weights and, at a few MB of them, by the fixed cost
 //   of a launch (about 3 us of barrier, TMEM and cluster set-up, pipeline fill
 //   and the last tile's way out). One B200, back to back, UE8M0: 1 x 4096 x 7168
-//   8.5 us (3.5 TB/s), 1 x 36864 x 7168 40.5 us (6.5 TB/s), 16 x 7168 x 2048 7.4
-//   us, 128 x 4096 x 7168 13.5 us; fp32 scales 8.5, 41, 7.4 and 15.2 us.
+//   8.9 us (3.3 TB/s), 1 x 36864 x 7168 40.5 us (6.5 TB/s), 16 x 7168 x 2048 6.5
+//   us, 128 x 4096 x 7168 13.6 us; fp32 scales 9.0, 41, 6.8 and 15.3 us.
 //
 // fp8_pair_kernel: many tokens. Two CTAs share a tile of 256 tokens (lanes) x
 //   256 weight rows (columns), each holding half of either operand; with fp32
@@ -27,8 +27,9 @@
 //   per thread and k-block. Bound by the tensor core at the clock that the power
 //   limit leaves (UE8M0), or by the way of a k-block's product through tensor
 //   memory and registers (fp32 scales). One B200, back to back, UE8M0: 4096 x
-//   4096 x 7168 87 us (2760 TFLOP/s), 16384 x 4096 x 7168 374 us, 8192 x 7168 x
-//   2048 94 us; fp32 scales 122 us (1970 TFLOP/s), 498 us and 140 us. Tiles of
+//   4096 x 7168 89 us (2700 TFLOP/s), 16384 x 4096 x 7168 375 to 393 us (by the
+//   clock), 8192 x 7168 x 2048 95 us; fp32 scales 122 us (1970 TFLOP/s), 505 us and
+//   138 us. Tiles of
 //   256 x 256 take an SM's shared memory 512 cycles per k-block for the 512 of its
 //   MMAs; 128 x 256 tiles of single CTAs would take 768.
 #include <atomic>
@@ -1526,8 +1527,8 @@ constexpr PlanCost kCost[2] = {
     {250, 1.7, 150, 2.5, 450, 8, 1250, 20, 580, 2400},  // fp32 scales
     {265, 0.3, 170, 0.4, 0, 15, 1100, 28, 275, 3400}};  // UE8M0
 
-// Both sides measured, UE8M0, one B200, back to back: 16 x 4096 x 7168 in 4
-// pieces 9.3 us, unsplit 17.4; 128 x 7168 x 2048 in tiles of 32 tokens 8.6 us,
+// Both sides measured, UE8M0, one B200, back to back: 16 x 4096 x 7168 in 8
+// pieces 9.5 us, in 4 9.3, unsplit 17.4; 128 x 7168 x 2048 in tiles of 32 tokens 8.6 us,
 // of 128 10.0, of 128 in two pieces 12.4; 512 x 4096 x 7168 as pairs 21.8 us, in
 // tiles of 128 22.0; 1024 x 4096 x 7168 25.4 and 38.8. fp32 scales: 512 x 4096 x
 // 7168 as pairs 37.1 us, in tiles of 128 29.2; 1024 x 4096 x 7168 39.2 and 55.4.
