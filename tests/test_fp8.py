@@ -53,6 +53,38 @@ def test_cpu_tensors_are_refused():
         fp8.quantize_blocks(torch.zeros(2, 128))
 
 
+def test_calls_run_on_their_operands_device(monkeypatch):
+    """With another device current, the call is made with the operands' device
+    current and on its current stream; a failing status raises."""
+    from kernelswift_b200 import fused_moe as fm
+
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    status = [0]
+    monkeypatch.setattr(fm, "_get_device", lambda: current[0])
+    monkeypatch.setattr(fm, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setitem(fm._bound, "moe_fp8_matmul",
+                        lambda *a: seen.append((current[0], a)) or status[0])
+    fm._enqueue("moe_fp8_matmul", 1, "x")
+    fm._enqueue("moe_fp8_matmul", 0, "y")
+    assert seen == [(1, ("x", 101)), (0, ("y", 100))] and current == [0]
+    status[0] = INVALID
+    with pytest.raises(_lib.MoeError):
+        fm._enqueue("moe_fp8_matmul", 1, "z")
+    assert current == [0]
+
+
 @pytest.mark.parametrize("fmt", ["fp32", "ue8m0"])
 def test_plan_covers_the_product(fmt):
     """Every plan's tiles cover the output, K splits leave no CTA empty and
