@@ -1521,7 +1521,7 @@ struct Plan {
 // CTAs on an SM, the bytes and columns of both (share, share_col). Its choice
 // was 1.02 times the best plan's time on average and 1.2 times at worst.
 struct PlanCost {
-  double kb, kb_col, share, share_col, tile, tile_col, split, split_col, pair_kb, pair_tile;
+  float kb, kb_col, share, share_col, tile, tile_col, split, split_col, pair_kb, pair_tile;
 };
 constexpr PlanCost kCost[2] = {
     {250, 1.7, 150, 2.5, 450, 8, 1250, 20, 580, 2400},  // fp32 scales
@@ -1532,39 +1532,40 @@ constexpr PlanCost kCost[2] = {
 // of 128 10.0, of 128 in two pieces 12.4; 512 x 4096 x 7168 as pairs 21.8 us, in
 // tiles of 128 22.0; 1024 x 4096 x 7168 25.4 and 38.8. fp32 scales: 512 x 4096 x
 // 7168 as pairs 37.1 us, in tiles of 128 29.2; 1024 x 4096 x 7168 39.2 and 55.4.
+// In 32 bits, which check_sizes allows, and by shifts: a call makes a plan.
 Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
-  const int64_t kbs = ceil_div(K, kKB);
+  const uint32_t tokens = uint32_t(T), blocks = uint32_t(ceil_div(N, kLanes));
+  const uint32_t kbs = uint32_t(ceil_div(K, kKB)), all = uint32_t(sms);
   const PlanCost& c = kCost[mx];
   Plan best = {0, 16, 1, 1};
-  double best_cost = 1e300;
-  for (int bn : {16, 32, 64, 128, 256}) {
-    if (bn == 256 && !mx) continue;
-    if (bn > 16 && bn / 2 >= T) continue;  // the half would hold every token
-    const int64_t tiles = ceil_div(T, bn) * ceil_div(N, kLanes);
-    const int occ = bn <= 64 ? 2 : 1;
+  float best_cost = INFINITY;
+  for (int lb = 4; lb <= (mx ? 8 : 7); ++lb) {
+    const uint32_t bn = 1u << lb;
+    if (lb > 4 && bn / 2 >= tokens) break;  // the half would hold every token
+    const uint32_t tiles = ((tokens + bn - 1) >> lb) * blocks;
+    const uint32_t occ = bn <= 64 ? 2 : 1;
     // clusters of other sizes leave SMs idle: 16 x 7168 x 18432 in 4 pieces
     // 24.3 us, in 5 28.6
-    for (int s = 1; s <= 8 && s <= kbs; s *= 2) {
-      const int64_t ctas = tiles * s;
-      if (s > 1 && ctas > int64_t(sms) * occ) break;
-      // 1 also for no tokens at all
-      const int64_t on_sm = ctas > sms ? occ : 1;
-      const double rounds = double(ceil_div(ctas, sms * on_sm));
-      const double kb =
-          std::max(c.kb + c.kb_col * bn, double(on_sm) * (c.share + c.share_col * bn));
-      const double cost = rounds * (double(ceil_div(kbs, s)) * kb + c.tile + c.tile_col * bn) +
-                          (s > 1 ? c.split + c.split_col * bn : 0);
+    for (int ls = 0; ls <= 3 && (1u << ls) <= kbs; ++ls) {
+      const uint32_t ctas = tiles << ls;
+      if (ls > 0 && ctas > all * occ) break;
+      const uint32_t on_sm = ctas > all ? occ : 1;
+      const float rounds = float((ctas + all * on_sm - 1) / (all * on_sm));
+      const float kb = std::max(c.kb + c.kb_col * bn, on_sm * (c.share + c.share_col * bn));
+      const float cost =
+          rounds * (float((kbs + (1u << ls) - 1) >> ls) * kb + c.tile + c.tile_col * bn) +
+          (ls > 0 ? c.split + c.split_col * bn : 0.0f);
       if (cost < best_cost) {
         best_cost = cost;
-        best = {0, bn, s, int(std::min<int64_t>(ctas, int64_t(sms) * occ))};
+        best = {0, int(bn), 1 << ls, int(std::min(ctas, all * occ))};
       }
     }
   }
-  if (T > 128) {
-    const int64_t tiles = ceil_div(T, 256) * ceil_div(N, 256);
-    const double rounds = double(ceil_div(tiles, sms / 2));
+  if (tokens > 128) {
+    const uint32_t tiles = ((tokens + 255) >> 8) * uint32_t(ceil_div(N, 256));
+    const float rounds = float((tiles + all / 2 - 1) / (all / 2));
     if (rounds * (kbs * c.pair_kb + c.pair_tile) < best_cost)
-      best = {1, 256, 1, int(2 * std::min<int64_t>(tiles, sms / 2))};
+      best = {1, 256, 1, int(2 * std::min(tiles, all / 2))};
   }
   return best;
 }
