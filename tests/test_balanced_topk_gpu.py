@@ -250,6 +250,18 @@ def test_captured_and_on_another_stream(cuda_device):
         check(logits, bias, w, ids, k, num_expert_group=8, topk_group=4)
 
 
+@pytest.mark.parametrize("E,G,kept", [(256, 8, 4), (384, 1, 1), (1024, 32, 9)])
+def test_bias_off_alignment(cuda_device, E, G, kept):
+    """A bias that is a slice of a larger tensor, strided or off a 16-byte boundary."""
+    logits, bias = inputs(40, E, torch.float32, 11)
+    x = logits.to(cuda_device)
+    wide = torch.zeros(2 * E + 1, device=cuda_device)
+    for view in (wide[1:E + 1], wide[1::2]):
+        view.copy_(bias)
+        w, ids = fm.balanced_topk(x, x, view, 8, num_expert_group=G, topk_group=kept)
+        check(logits, bias, w, ids, 8, num_expert_group=G, topk_group=kept)
+
+
 @pytest.mark.parametrize("score,renorm", [("sigmoid", True), ("softmax", False)])
 def test_captured_training_step(cuda_device, score, renorm):
     T, E, k = 70, 64, 6
