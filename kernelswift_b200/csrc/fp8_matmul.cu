@@ -151,8 +151,14 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 
-// The stages that the producers have filled, and the parity of each one's last
-// fill (whichever warp's), so that they can wait for the copies before they end.
+// The slots of a ring that have been filled, and the parity of each one's last
+// fill (whichever warp's), so that a block ends only after what it caused: the
+// copies into a stage (drain), and the MMAs' last arrivals on the ring's `empty`
+// barriers (released). tcgen05.commit arrives asynchronously, for a CTA pair on
+// the other CTA's barriers too; the MMAs' completion alone (final_bar) does not say
+// that earlier arrivals have landed, and one that came late would land in the
+// shared memory of the SM's next block. A slot's k-th fill and its k-th release
+// complete phases of one parity. When a wait gave up, `released` does not wait.
 struct Filled {
   uint32_t used = 0, parity = 0;
   __device__ __forceinline__ void add(int stage, uint32_t phase) {
@@ -160,11 +166,13 @@ struct Filled {
     parity = (parity & ~(1u << stage)) | (phase << stage);
   }
   __device__ __forceinline__ void drain(uint64_t* full, int stages, uint64_t limit) const {
-    for (int s = 0; s < stages; ++s)
-      if ((used >> s) & 1u) {
-        volatile int no_abort = 0;
-        mbar_wait_bounded(&full[s], (parity >> s) & 1u, &no_abort, limit);
-      }
+    volatile int no_abort = 0;
+    released(full, stages, &no_abort, limit);
+  }
+  __device__ __forceinline__ void released(uint64_t* bars, int slots, volatile int* abort,
+                                           uint64_t limit) const {
+    for (int s = 0; s < slots; ++s)
+      if ((used >> s) & 1u) mbar_wait_bounded(&bars[s], (parity >> s) & 1u, abort, limit);
   }
 };
 
@@ -495,6 +503,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
       }
     }
     filled.drain(full, STAGES, limit);
+    filled.released(empty, STAGES, abort_flag, limit);
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     // The whole warp walks the loop and one lane issues: operands computed by
@@ -616,6 +625,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
         ww.fetch(static_cast<const uint8_t*>(p.ws) + int64_t(tile.n) * p.kb_total, true, lane, q0,
                  p.kb_total);
       };
+      Filled filled;
       if (first < tiles) fetch(first, q_first);
       for (int i = first; ok && i < tiles; i += step) {
         for (int q0 = q_first; q0 < q_end; q0 += Q) {
@@ -629,6 +639,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(&sfull[slot]);
+          filled.add(slot, sphase);
           // the next words' loads run while the slots ahead are used
           if (q0 + Q < q_end)
             fetch(i, q0 + Q);
@@ -640,6 +651,7 @@ __global__ void __launch_bounds__(ColsCfg<MX, BN>::kThreads, ColsCfg<MX, BN>::kC
           }
         }
       }
+      filled.released(sempty, SLOTS, abort_flag, limit);
     } else {
       // sx * sw of four k-blocks at a time, loaded together and a turn ahead
       constexpr int R = (BN + 31) / 32, U = 4;
@@ -1166,6 +1178,7 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
     // the even CTA's barriers count both CTAs' bytes; the odd CTA stays until
     // the cluster barrier below
     if (rank == 0) filled.drain(full, STAGES, limit);
+    filled.released(empty, STAGES, abort_flag, limit);
   } else if (warp >= 1 && warp <= C::kHalves && rank == 0) {
     // ---------------- MMA issuers, for both CTAs ----------------
     // The whole warp walks the loop and one lane issues: operands computed by
@@ -1294,6 +1307,7 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
     int slot = 0;
     uint32_t sphase = 0;
     bool ok = true;
+    Filled filled;
     if (first < tiles) fetch(first, 0);
     for (int i = first; ok && i < tiles; i += step) {
       for (int q0 = 0; q0 < quads; q0 += Q) {
@@ -1308,6 +1322,7 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&sfull[slot]), 0));
+        filled.add(slot, sphase);
         // the next words' loads run while the slots ahead are used
         if (q0 + Q < quads)
           fetch(i, q0 + Q);
@@ -1319,6 +1334,7 @@ __global__ void __launch_bounds__(PairCfg<MX, VEC>::kThreads, 1)
         }
       }
     }
+    filled.released(sempty, C::kSfSlots, abort_flag, limit);
   } else if (warp >= 4) {
     // ---------------- promotion and epilogue of this CTA's 128 tokens ----------------
     if constexpr (!MX) setmaxnreg_inc<C::kEpiRegs>();

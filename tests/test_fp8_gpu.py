@@ -396,6 +396,25 @@ def test_same_bits_every_time_and_captured(cuda_device):
                 assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_products_right_behind_each_other(cuda_device, fmt):
+    """A product's last arrivals are on barriers of its own shared memory: the
+    products launched behind it, which take the same memory for theirs, give the
+    same bits every time."""
+    sizes = [(2048, 1280, 640), (20, 512, 1000), (1300, 2403, 520), (1, 1024, 2000)]
+    plans = [fp8.block_matmul_plan(*size, fmt)["cta_pairs"] for size in sizes]
+    assert plans == [1, 0, 1, 0]
+    work = [operands(*size, fmt, cuda_device, 5) for size in sizes]
+    want = []
+    for x, w in work:
+        want.append(fp8.block_matmul(*x, *w))
+        torch.cuda.synchronize()
+        check_product(want[-1], x, w)
+    got = [[fp8.block_matmul(*x, *w) for x, w in work] for _ in range(60)]
+    for outs in got:
+        assert all(torch.equal(g, v) for g, v in zip(outs, want))
+
+
 # ---------------------------------------------------------------------------
 # the MLP, and the layer: balanced routing, routed experts, shared expert
 # ---------------------------------------------------------------------------
