@@ -191,11 +191,14 @@ __device__ __forceinline__ void top_two(double v, double& a, double& b) {
   a = fmax(a, v);
 }
 
-// Bit g * lanes_per_group: group g is kept. Sets `close` when the choice hung on
-// less than `tol` (given the value of the last group kept).
-template <typename R, int PL, typename Tol>
+// Bit g * lanes_per_group: group g is kept. Groups are compared by half their
+// value, which stays in range where two of the type's lowest numbers are added.
+// err(m) bounds the error of half a value whose terms' halves have magnitudes that
+// add up to m: the terms may cancel, and their roundings do not. Sets `close` when
+// the bounds of a group left out and of the last one kept meet.
+template <typename R, int PL, typename Err>
 __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R (&c)[PL],
-                                                int lane, R* scratch, Tol tol, bool& close) {
+                                                int lane, R* scratch, Err err, bool& close) {
   const int per = p.lanes_per_group;
   const int g = lane >> p.group_shift, sub = lane & (per - 1);
   R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
@@ -223,7 +226,9 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
     top_two(oa, a, b);
     top_two(ob, a, b);
   }
-  R value = p.top2 && p.EG > 1 ? a + b : a;  // a group of one has no second
+  if (!p.top2 || p.EG == 1) b = R(0);  // a group of one has no second
+  const R ha = R(0.5) * a, hb = R(0.5) * b;
+  R value = ha + hb;
   if (value != value) value = R(-INFINITY);  // +inf and -inf in one group
   // a group's rank: how many come before it
   int rank = 0;
@@ -233,10 +238,12 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
   }
   const bool mine = g < p.G && sub == 0;
   const bool keep = mine && rank < p.kept;
+  // infinite values are exact: their bounds are NaN or on the far side
+  const R e = err(fabs(ha) + fabs(hb));
   const R last =
-      __shfl_sync(0xffffffffu, value,
+      __shfl_sync(0xffffffffu, value - e,
                   __ffs(__ballot_sync(0xffffffffu, mine && rank == p.kept - 1)) - 1);
-  close = mine && !keep && value >= last - tol(last) && last > R(-INFINITY);
+  close = mine && !keep && value + e >= last;
   return __ballot_sync(0xffffffffu, keep);
 }
 // Bit j: this lane's expert j exists and its group is kept.
@@ -368,11 +375,12 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   auto tol = [&](float v) { return scores + 2.0f * 2.0f * (PL + 0.5f) * 0x1p-23f * fabsf(v); };
   uint32_t kept = 0xffffffffu;
   if (p.G > 1) {
-    // a value is the sum of two uncut c, rounded once more
+    // half a value is off by the error of one score, half an ulp of each (halved)
+    // term, lost when its bias was added, and as much at most for their sum; twice that
     bool close = false;
     kept = kept_groups(
         p, c, lane, reinterpret_cast<float*>(scratch),
-        [&](float v) { return 2.0f * scores + 2.0f * 2.0f * 1.5f * 0x1p-23f * fabsf(v); }, close);
+        [&](float m) { return 0.5f * scores + 2.0f * 2.0f * 0x1p-24f * m; }, close);
     if (__any_sync(0xffffffffu, close)) kept = kept_exact<PL>(p, row, mx, lane, scratch);
   }
   constexpr uint32_t kLow = PL - 1;

@@ -117,6 +117,46 @@ def test_masked_experts_and_empty_rows(cuda_device, score, G, kept):
         assert torch.isfinite(w).all()
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("G,per,kept", [(8, 2, 4), (32, 2, 8), (16, 4, 5)])
+def test_groups_of_opposite_biases(cuda_device, G, per, kept, score):
+    """A group's two largest nearly cancel: their sum is far smaller than what
+    each lost when its bias was added in 32 bits. Biases of 1e2 to 1e5, and
+    ordinary ones against scores that are small themselves."""
+    T, k = 2048, 4
+    sign = torch.ones(G, per)
+    sign[:, 1] = -1
+    sign[:, 2:] = -2
+    for size, mean in ((1e2, 0), (1e3, 0), (1e4, 0), (1e5, 0), (0.25, -16), (1.0, -16), (8.0, -12)):
+        logits, _ = inputs(T, G * per, torch.float32, int(size) + G)
+        logits += mean
+        bias = (size * sign).reshape(-1)
+        x = logits.to(cuda_device)
+        kw = dict(num_expert_group=G, topk_group=kept, scoring_func=score)
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, **kw)
+        check(logits, bias, w, ids, k, **kw)
+
+
+@pytest.mark.parametrize("G,kept", [(1, 1), (8, 3), (5, 2)])
+def test_biases_of_the_lowest_value(cuda_device, G, kept):
+    """Experts masked by the lowest value of fp32 or bf16, of which groups have
+    one, two or only such: sums past 32 bits' range keep their 64-bit order."""
+    T, E, k = 60, 40, 6
+    logits, bias = inputs(T, E, torch.float32, 2)
+    low, bf = torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min
+    for masked in ({0: low, 3: low, 4: low}, {e: low for e in range(0, 20)},
+                   {e: (low, bf, -torch.inf)[e % 3] for e in range(2, 40)},
+                   {e: (low, bf)[e // 5 % 2] for e in range(40)}):
+        b = bias.clone()
+        for e, v in masked.items():
+            b[e] = v
+        x = logits.to(cuda_device)
+        for group_score in ("top2", "max"):
+            kw = dict(num_expert_group=G, topk_group=kept, group_score=group_score)
+            w, ids = fm.balanced_topk(x, x, b.to(cuda_device), k, **kw)
+            check(logits, b, w, ids, k, **kw)
+
+
 def test_nan_ranks_last_and_ids_stay_valid(cuda_device):
     x = torch.randn(4, 16, device=cuda_device)
     x[0, 3] = torch.nan
