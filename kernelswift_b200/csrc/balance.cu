@@ -110,7 +110,8 @@ __device__ __forceinline__ double score_rcp(double x) { return 1.0 / x; }
 // exp, the difference l - max 0.2, the reciprocal and the product 1.5, and the
 // error of the sum, which the terms at distance d share in by their weight: their
 // mean d is at most ln 1024 < 7, so 9 for the terms, and half an ulp for each of
-// the PL + 4 additions.
+// the PL + 4 additions. To this the caller adds 2^-126: results below it are flushed
+// to 0.
 template <int PL>
 __device__ __forceinline__ float score_ulps(int softmax, float mx) {
   return softmax ? 16.0f + 0.5f * (PL + 4) : 6.0f + 1.2f * fmaxf(-mx, 0.0f);
@@ -371,7 +372,7 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   biased_scores<float, PL, Tin>(p, l, mx, lane, c, smax);
   // of a difference of two c: both scores, the rounding of both sums with the
   // bias and the bits cut off both keys; twice that, since it is itself rounded
-  const float scores = 2.0f * 2.0f * score_ulps<PL>(p.softmax, mx) * 0x1p-23f * smax;
+  const float scores = 2.0f * 2.0f * (score_ulps<PL>(p.softmax, mx) * 0x1p-23f * smax + 0x1p-126f);
   auto tol = [&](float v) { return scores + 2.0f * 2.0f * (PL + 0.5f) * 0x1p-23f * fabsf(v); };
   uint32_t kept = 0xffffffffu;
   if (p.G > 1) {

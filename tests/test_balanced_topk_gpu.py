@@ -157,6 +157,20 @@ def test_biases_of_the_lowest_value(cuda_device, G, kept):
             check(logits, b, w, ids, k, **kw)
 
 
+@pytest.mark.parametrize("G,kept", [(1, 1), (4, 2)])
+def test_scores_below_the_normal_range(cuda_device, G, kept):
+    """Logits whose sigmoids lie about 2^-126, with biases of that size: the
+    fast 32-bit scores are 0 there, the order is still that of 64 bits."""
+    T, E, k = 300, 64, 8
+    g = torch.Generator().manual_seed(7)
+    logits = -87.5 + 0.5 * torch.randn(T, E, generator=g)
+    bias = 1e-38 * torch.randn(E, generator=g)
+    x = logits.to(cuda_device)
+    kw = dict(num_expert_group=G, topk_group=kept)
+    _, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, **kw)
+    assert torch.equal(ids.cpu().long(), orc.balanced_topk(logits, bias, k, **kw)[1])
+
+
 def test_nan_ranks_last_and_ids_stay_valid(cuda_device):
     x = torch.randn(4, 16, device=cuda_device)
     x[0, 3] = torch.nan
