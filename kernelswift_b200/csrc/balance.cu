@@ -557,11 +557,12 @@ __global__ void __launch_bounds__(32 * kWarps)
     Tin* out = static_cast<Tin*>(p.grad_logits) + t * p.E;
     const bool mine = lane < p.k;
     const int64_t at = t * p.k + lane;
-    int e = 0;
+    int64_t id = -1;
     if (mine)
-      e = p.ids64 ? int(static_cast<const int64_t*>(p.ids)[at])
-                  : static_cast<const int32_t*>(p.ids)[at];
-    const bool valid = mine && e >= 0 && e < p.E;  // an id out of range has no gradient
+      id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at]
+                   : static_cast<const int32_t*>(p.ids)[at];
+    const bool valid = id >= 0 && id < p.E;  // an id out of range has no gradient
+    const int e = valid ? int(id) : 0;
     const float l = valid ? to_f32(row[e]) : -INFINITY;
     const float g = valid ? p.scale * p.grad_weights[at] : 0.0f;
     float d = 0.0f;     // this lane's entry

@@ -272,6 +272,36 @@ def test_gradient_against_differences(cuda_device):
                     assert abs(x.grad[t, e].item() - diff.item()) < 1e-9 + 8 * RTOL
 
 
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("renorm", [0, 1])
+def test_gradient_of_ids_out_of_range(cuda_device, score, renorm):
+    """Through the C entry: such an id contributes nothing, in either width.
+    2^32 + 3 is 3 in its low 32 bits."""
+    from kernelswift_b200 import _lib
+    from kernelswift_b200.fused_moe import _ptr, _stream
+
+    T, E, k = 5, 24, 4
+    x, _ = inputs(T, E, torch.float32, 6)
+    gw = torch.randn(T, k, generator=torch.Generator().manual_seed(2))
+    good = torch.tensor([7, 11, 0, 23])
+    for dtype, code, bad in ((torch.int64, _lib.DT_I64, (-1, E, 2 ** 32 + 3, -2 ** 32 + 3)),
+                             (torch.int32, _lib.DT_I32, (-1, E, 2 ** 31 - 1, -2 ** 31))):
+        for at, wrong in enumerate(bad):
+            ids = good.repeat(T, 1)
+            ids[1:, at] = wrong
+            dev = [t.to(cuda_device) for t in (x, ids.to(dtype), gw)]
+            grad = torch.full((T, E), 9.0, device=cuda_device)
+            _lib.call("moe_balanced_topk_backward", _ptr(dev[0]), _lib.DT_F32, _ptr(dev[1]), code,
+                      _ptr(dev[2]), T, E, k, renorm, score, 1.5, _ptr(grad), _stream(cuda_device))
+            name = "sigmoid" if score else "softmax"
+            rest = [j for j in range(k) if j != at]
+            want = formula(x, None, gw[:, rest], k - 1, name, bool(renorm), 1.5, ids[:, rest])
+            whole = formula(x, None, gw, k, name, bool(renorm), 1.5, good.repeat(T, 1))
+            want[0] = whole[0]
+            room = RTOL * 1.5 * gw.abs().amax(1, keepdim=True).double() * k
+            assert ((grad.double().cpu() - want).abs() <= room).all(), wrong
+
+
 def test_gradient_of_expanded_logits(cuda_device):
     row = torch.randn(1, 16, device=cuda_device, requires_grad=True)
     x = row.expand(6, 16)
