@@ -75,30 +75,33 @@ def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, inde
     _no_grad_needed("out", out)
 
 
-def _addend(addend: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype, index: int):
+def _addend(addend: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, index: int,
+            out: torch.Tensor):
     """(pointer, row stride) of the addend."""
     _no_grad_needed("addend", addend)
     if addend.shape != (rows, cols) or addend.dtype != dtype or addend.get_device() != index:
         raise ValueError(f"addend must be a {dtype} [{rows}, {cols}] tensor on the operands' "
                          "device")
-    if addend.numel() and (addend.stride(1) != 1 or addend.stride(0) < cols and rows > 1):
+    if addend.numel() and (addend.stride(1) != 1 and cols > 1
+                           or addend.stride(0) < cols and rows > 1):
         raise ValueError("addend must have dense rows")
+    _check_apart(out, addend)
     return addend.data_ptr(), max(addend.stride(0), cols)
 
 
 def _check_apart(out: torch.Tensor, addend: torch.Tensor) -> None:
     """out and addend are the same elements or share none: an element is read by
-    the thread that writes it, and only just before."""
-    size, cols, pitch = out.element_size(), out.shape[1], out.stride(0)
+    the thread that writes it, and only just before. Strides of a single row or
+    column mean nothing."""
+    size, (rows, cols) = out.element_size(), out.shape
     apart = (addend.data_ptr() - out.data_ptr()) // size
-    if not out.numel() or apart == 0 and out.stride() == addend.stride():
+    pitch, add_pitch = (t.stride(0) if rows > 1 else cols for t in (out, addend))
+    if not out.numel() or apart == 0 and pitch == add_pitch:
         return
-    if apart >= (out.shape[0] - 1) * pitch + cols:
-        return
-    if -apart >= (out.shape[0] - 1) * addend.stride(0) + cols:
+    if apart >= (rows - 1) * pitch + cols or -apart >= (rows - 1) * add_pitch + cols:
         return
     # columns of one wider matrix
-    if addend.stride(0) == pitch and cols <= apart % pitch <= pitch - cols:
+    if add_pitch == pitch and cols <= apart % pitch <= pitch - cols:
         return
     raise ValueError("out and addend overlap without being the same elements")
 
@@ -210,9 +213,7 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         out_dtype = out.dtype
         _check_out(out, T, N, out_dtype, index)
         ld_out = max(out.stride(0), N)
-        if addend is not None:
-            _check_apart(out, addend)
-    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, N, out_dtype, index)
+    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, N, out_dtype, index, out)
     if x_scale.requires_grad or w_scale.requires_grad:
         _no_grad_needed("x_scale", x_scale)
         _no_grad_needed("w_scale", w_scale)
@@ -281,9 +282,7 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     else:
         _check_out(out, T, H, x.dtype, index)
-        if addend is not None:
-            _check_apart(out, addend)
-    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, H, x.dtype, index)
+    add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, H, x.dtype, index, out)
     code = _DTYPE_CODE[x.dtype]
     # of its own: a workspace kept by stream would be shared by captured graphs
     ws = torch.empty(_mlp_workspace_bytes(T, H, inter, code, fmt), dtype=torch.uint8,

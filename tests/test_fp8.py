@@ -85,6 +85,58 @@ def test_calls_run_on_their_operands_device(monkeypatch):
     assert current == [0]
 
 
+def apart(out, addend):
+    """Whether fp8 takes `addend` for `out`."""
+    try:
+        fp8._addend(addend, *out.shape, out.dtype, -1, out)
+    except ValueError:
+        return False
+    return True
+
+
+def test_a_single_row_or_column_in_place():
+    """The strides of one row, or one column, mean nothing."""
+    buf = torch.zeros(8, 80)
+    one = buf[:1, :64]
+    assert apart(one, one) and apart(one, buf[0, :64].unsqueeze(0))  # strides 80 and 64
+    assert apart(one, buf[0, 64:].repeat(4)[None]) and not apart(one, buf[0, 1:65].unsqueeze(0))
+    row = torch.as_strided(buf, (1, 64), (0, 1), 0)
+    assert apart(row, row) and apart(row, one) and apart(one, row)
+    assert not apart(row, torch.as_strided(buf, (1, 64), (0, 1), 63))
+    assert apart(row, torch.as_strided(buf, (1, 64), (0, 1), 64))
+    column = torch.as_strided(buf, (8, 1), (80, 8), 3)
+    assert apart(column, column) and apart(column, buf[:, 3:4]) and apart(column, buf[:, 4:5])
+    assert not apart(column, torch.as_strided(buf, (8, 1), (40, 1), 3))
+
+
+def test_overlaps_are_refused():
+    """Every accepted pair of layouts is the same elements or shares none; the
+    same elements, columns of one matrix and runs behind each other are accepted."""
+    import random
+
+    rng, buf = random.Random(5), torch.zeros(400)
+    taken = 0
+    for _ in range(4000):
+        rows, cols = rng.choice((1, 1, 2, 3, 5)), rng.choice((1, 2, 4, 7))
+        def view():
+            strides = (rng.choice((0, cols, cols, cols + 1, 2 * cols, 16)), rng.choice((1, 1, 1, 3)))
+            return torch.as_strided(buf, (rows, cols), strides, rng.randint(0, 40))
+        out, addend = view(), view()
+        if rows > 1 and out.stride(0) < cols or cols > 1 and out.stride(1) != 1:
+            continue  # not an output
+        cells = []
+        for t in (out, addend):
+            cells.append([t.storage_offset() + r * t.stride(0) + c * t.stride(1)
+                          for r in range(rows) for c in range(cols)])
+        if apart(out, addend):
+            taken += 1
+            assert cells[0] == cells[1] or not set(cells[0]) & set(cells[1])
+        else:
+            dense = (rows == 1 or addend.stride(0) >= cols) and (cols == 1 or addend.stride(1) == 1)
+            assert not dense or cells[0] != cells[1]
+    assert taken > 500
+
+
 @pytest.mark.parametrize("fmt", ["fp32", "ue8m0"])
 def test_plan_covers_the_product(fmt):
     """Every plan's tiles cover the output, K splits leave no CTA empty and

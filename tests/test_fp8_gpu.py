@@ -498,6 +498,19 @@ def test_addend_beside_the_output(cuda_device):
         assert torch.equal(buf[:, to:to + 64], want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_one_token_added_in_place(cuda_device, fmt):
+    """A row of a wider buffer as output and, under another stride, as addend."""
+    x, w = operands(1, 64, 256, fmt, cuda_device)
+    buf = gen(3, 80, dtype=torch.bfloat16).to(cuda_device)
+    want = fp8.block_matmul(*x, *w, addend=buf[1:2, :64].clone())
+    before = buf.clone()
+    got = fp8.block_matmul(*x, *w, out=buf[1:2, :64], addend=buf[1, :64].unsqueeze(0))
+    assert torch.equal(got, want)
+    before[1, :64] = want[0]
+    assert torch.equal(buf, before)
+
+
 def test_refusals(cuda_device):
     x, w = operands(4, 64, 256, "fp32", cuda_device)
     xu, wu = operands(4, 64, 256, "ue8m0", cuda_device)
