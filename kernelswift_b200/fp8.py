@@ -10,7 +10,9 @@ formats per expert.
 
 Everything runs in libmoe_b200.so on the current stream of the operands'
 device; nothing allocates but the outputs, and a call can be captured in a
-CUDA graph. There is no CPU path and no gradient: these are serving operators.
+CUDA graph. There is no CPU path and no gradient: these are serving operators,
+which refuse operands that need one or carry a tangent (quantize_blocks takes
+weights that need a gradient as they are).
 """
 from __future__ import annotations
 
@@ -18,9 +20,10 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .fused_moe import _check_cuda, _DTYPE_CODE, _enqueue
+from .fused_moe import _check_cuda, _DTYPE_CODE, _enqueue, _refuse_tangents
 
 _FORMAT = {"fp32": 0, "ue8m0": 1}
 _SCALE_FORMAT = {torch.float32: 0, torch.uint8: 1}
@@ -133,6 +136,8 @@ def quantize_rows(x: torch.Tensor, scale_format: str = "ue8m0", gated: bool = Fa
         raise ValueError("x must be a 2-D f32/f16/bf16 tensor, of an even width when gated")
     if x.requires_grad:
         _no_grad_needed("x", x)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x=x)
     x = _rows_of(x)
     T, wide = x.shape
     K = wide // 2 if gated else wide
@@ -161,6 +166,8 @@ def quantize_blocks(w: torch.Tensor, scale_format: str = "ue8m0"
         raise ValueError(f"scale_format must be one of {sorted(_FORMAT)}")
     if w.dim() != 2 or w.dtype not in _FLOAT or w.numel() == 0:
         raise ValueError("w must be a 2-D f32/f16/bf16 tensor")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(w=w)
     w = _rows_of(w.detach())
     N, K = w.shape
     dev = w.device
@@ -193,6 +200,8 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
             _check_cuda(name, t)
         raise ValueError("x, x_scale, w and w_scale must be on one device")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x=x, x_scale=x_scale, w=w, w_scale=w_scale, addend=addend, out=out)
     x, w = _fp8_rows("x", x), _fp8_rows("w", w)
     (T, K), (N, w_cols) = x.shape, w.shape
     kb, nb = (K + 127) // 128, (N + 127) // 128
@@ -260,6 +269,9 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
                         ("w2_scale", w2_scale)):
             _check_cuda(name, t)
         raise ValueError("x and the weights with their scales must be on one device")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x=x, w13=w13, w13_scale=w13_scale, w2=w2, w2_scale=w2_scale,
+                         addend=addend, out=out)
     for name, t in (("x", x), ("w13_scale", w13_scale), ("w2_scale", w2_scale)):
         if t.requires_grad:
             _no_grad_needed(name, t)

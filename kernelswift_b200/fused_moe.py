@@ -23,6 +23,7 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -75,6 +76,14 @@ def _enqueue(entry: str, index: int, *args) -> None:
             status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status, entry)
+
+
+def _refuse_tangents(**operands: torch.Tensor | None) -> None:
+    """Forward-mode differentiation reaches no kernel of the library: an operand
+    that carries a tangent would lose it. Asked for only while a level is open."""
+    for name, t in operands.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent; this operator has no forward-mode derivative")
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -248,12 +257,16 @@ def balanced_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     they all vanish) and scaled. Returns (topk_weights [T, k], topk_ids [T, k]).
 
     expert_load: int32 [E]; the number of tokens that chose each expert is
-    added to it (what a training loop adjusts the bias by).
+    added to it (what a training loop adjusts the bias by). Each run of the
+    forward pass adds: under activation checkpointing, which runs it again for
+    the backward pass, route outside the checkpointed part or halve the counts.
 
-    The weights are differentiable with respect to `gating_output`; the
-    choice and the bias have no gradient.
+    The weights are differentiable with respect to `gating_output` (backward
+    mode, once; a tangent is refused); the choice and the bias have no gradient.
     """
     _check_cuda("gating_output", gating_output)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(gating_output=gating_output)
     if gating_output.dim() != 2 or gating_output.shape[0] != hidden_states.shape[0]:
         raise ValueError("gating_output must be [T, E] with T = hidden_states.shape[0]")
     if scoring_func not in _SCORING:

@@ -392,6 +392,22 @@ def test_offsets_past_32_bits(cuda_device):
     assert not grad[6:T - 2].any()
 
 
+def test_forward_mode_is_refused(cuda_device):
+    """A tangent of the logits would be lost; one of the bias has no effect."""
+    import torch.autograd.forward_ad as fwd
+
+    x, bias = (t.to(cuda_device) for t in inputs(4, 16, torch.float32, 1))
+    want = fm.balanced_topk(x, x, bias, 2)
+    with fwd.dual_level():
+        for logits in (x, x.clone().requires_grad_()):
+            with pytest.raises(ValueError, match="forward"):
+                fm.balanced_topk(x, fwd.make_dual(logits, torch.ones_like(x)), bias, 2)
+        got = fm.balanced_topk(x, x, fwd.make_dual(bias, torch.ones_like(bias)), 2)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+    with pytest.raises(ValueError, match="forward"):
+        torch.func.jvp(lambda l: fm.balanced_topk(x, l, None, 2)[0], (x,), (x,))
+
+
 def test_refusals(cuda_device):
     from kernelswift_b200._lib import MoeError
 

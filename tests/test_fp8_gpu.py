@@ -511,6 +511,32 @@ def test_one_token_added_in_place(cuda_device, fmt):
     assert torch.equal(buf, before)
 
 
+def test_forward_mode_is_refused(cuda_device):
+    """No tangent is lost silently."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w = operands(4, 64, 256, "fp32", cuda_device)
+    w13, w2 = operands(1, 256, 64, "fp32", cuda_device)[1], operands(1, 64, 128, "fp32", cuda_device)[1]
+    rows = gen(4, 64).to(cuda_device)
+    add = gen(4, 64, dtype=torch.bfloat16).to(cuda_device)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: fp8.quantize_rows(dual(rows)), lambda: fp8.quantize_blocks(dual(rows)),
+                     lambda: fp8.block_matmul(x[0], dual(x[1]), *w),
+                     lambda: fp8.block_matmul(*x, w[0], dual(w[1])),
+                     lambda: fp8.block_matmul(*x, *w, addend=dual(add)),
+                     lambda: fp8.block_matmul(*x, *w, out=dual(add)),
+                     lambda: fp8.swiglu_mlp(dual(rows), *w13, *w2),
+                     lambda: fp8.swiglu_mlp(rows, w13[0], dual(w13[1]), *w2),
+                     lambda: fp8.swiglu_mlp(rows, *w13, w2[0], dual(w2[1])),
+                     lambda: fp8.swiglu_mlp(rows, *w13, *w2, addend=dual(rows))):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+        fp8.block_matmul(*x, *w, addend=add)
+
+
 def test_refusals(cuda_device):
     x, w = operands(4, 64, 256, "fp32", cuda_device)
     xu, wu = operands(4, 64, 256, "ue8m0", cuda_device)
