@@ -1,5 +1,9 @@
 """CPU: refusals of the dense fp8 entry points (on the host, before any
 launch), the plan of the product, and the oracle's roundings."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -51,6 +55,26 @@ def test_cpu_tensors_are_refused():
         fp8.quantize_rows(torch.zeros(2, 128))
     with pytest.raises(ValueError):
         fp8.quantize_blocks(torch.zeros(2, 128))
+
+
+def test_import_with_a_torch_without_cuda():
+    """The host's queries need no CUDA in torch, and tensors are refused as ever."""
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+from kernelswift_b200 import fp8, fused_moe as fm
+assert fm.fused_experts_plan(16, 256, 128, 8, 2)
+assert fp8.block_matmul_plan(1, 128, 128)["splits"] == 1
+try:
+    fm.balanced_topk(torch.zeros(2, 8), torch.zeros(2, 8), None, 2)
+except ValueError:
+    print("refused")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1],
+                          capture_output=True, text=True, timeout=300)
+    assert done.stdout == "refused\n", done.stderr[-2000:]
 
 
 def test_calls_run_on_their_operands_device(monkeypatch):
