@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from kernelswift_b200 import _lib, fp8
+from fp8_plans import CASES, PLANS
 from oracle import moe_oracle as orc
 
 F32, BF16, I8 = _lib.DT_F32, _lib.DT_BF16, _lib.DT_I8
@@ -181,6 +182,35 @@ def test_plan_covers_the_product(fmt):
                 else:
                     assert 1 <= p["ctas"] <= min(tiles, 296)
     assert fp8.block_matmul_plan(0, 64, 64, fmt)["ctas"] == 0
+
+
+def plan_of(T, N, K, fmt):
+    p = fp8.block_matmul_plan(T, N, K, fmt)
+    return p["cta_pairs"], p["tile_cols"], p["splits"]
+
+
+def test_listed_sizes_take_their_plans():
+    for fmt, plan, size in CASES:
+        assert plan_of(*size, fmt) == plan, (fmt, size)
+        T, N, K = size
+        assert T % (256 if plan[0] else plan[1]) and N % (256 if plan[0] else 128) and K % 128
+
+
+@pytest.mark.parametrize("fmt", ["fp32", "ue8m0"])
+def test_no_plan_goes_unlisted(fmt):
+    """Every plan that sizes drawn over the whole range take is one that the GPU
+    tests run."""
+    import math
+    import random
+
+    rng, seen = random.Random(2), set()
+
+    def draw(lo, hi):
+        return int(math.exp(rng.uniform(math.log(lo), math.log(hi))))
+
+    for _ in range(60000):
+        seen.add(plan_of(draw(1, 30000), draw(1, 60000), draw(1, 60000), fmt))
+    assert seen == set(PLANS[fmt])
 
 
 def test_oracle_roundings():

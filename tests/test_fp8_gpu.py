@@ -9,6 +9,7 @@ import torch
 
 from kernelswift_b200 import fp8
 from kernelswift_b200 import fused_moe as fm
+from fp8_plans import CASES
 from oracle import moe_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -206,6 +207,46 @@ def test_product(cuda_device, T, N, K, fmt):
     check_product(want, x, w, add)
     got = fp8.block_matmul(*x, *w, addend=add, out=add)  # in place
     assert got is add and torch.equal(got, want)
+
+
+def dense64(x, w):
+    """orc.fp8_dense on the GPU, in torch's fp64: (product, sum of magnitudes)."""
+    def values(s):
+        return torch.exp2(s.double() - 127) if s.dtype == torch.uint8 else s.double()
+
+    (T, K), N = x[0].shape, w[0].shape[0]
+    a = x[0].double() * values(x[1]).repeat_interleave(128, 1)[:, :K]
+    b = w[0].double() * (values(w[1]).repeat_interleave(128, 0)[:N]
+                         .repeat_interleave(128, 1)[:, :K])
+    return a @ b.t(), a.abs() @ b.abs().t()
+
+
+@pytest.mark.parametrize("fmt,plan,size", CASES)
+def test_every_plan(cuda_device, fmt, plan, size):
+    """Each tile and split, plain and with an addend, into a tensor of its own, in
+    place and into columns of a wider one; bounds as in check_product."""
+    T, N, K = size
+    x, w = operands(T, N, K, fmt, cuda_device, 11)
+    want, mag = dense64(x, w)
+
+    def check(out, add=0.0):
+        room = (HALF[out.dtype] * (want + add).abs()
+                + (4 + K / 32) * 2.0 ** -23 * (mag + abs(add)))
+        tiny = 2.0 ** -25 if out.dtype == torch.float16 else 0.0
+        err = (out.double() - want - add).abs()
+        assert (err <= room + tiny).all(), (err - room).max()
+
+    check(fp8.block_matmul(*x, *w, out_dtype=torch.float32))
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        add = gen(T, N, seed=5, dtype=dtype).to(cuda_device)
+        got = fp8.block_matmul(*x, *w, addend=add, out_dtype=dtype)
+        check(got, add.double())
+        wide = torch.full((T + 1, N + 16), 7.0, dtype=dtype, device=cuda_device)
+        inner = wide[:-1, 8:N + 8]
+        inner.copy_(add)
+        assert torch.equal(fp8.block_matmul(*x, *w, addend=inner, out=inner), got)
+        assert (wide[-1] == 7).all() and (wide[:, :8] == 7).all() and (wide[:, N + 8:] == 7).all()
+        assert torch.equal(fp8.block_matmul(*x, *w, addend=add, out=add), got)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
