@@ -95,6 +95,67 @@ def test_gated_scale_next_to_a_power_of_two(cuda_device):
     assert torch.equal(orc.fp8_scale_values(s.cpu()), want)
 
 
+MANY = [(2500, 1030, 0),   # rows off 16-byte boundaries in every type
+        (1300, 2048, 0),   # aligned, whole runs
+        (1200, 2303, 3),   # the first row too, and the last run partial
+        (9500, 200, 1)]    # less than a run
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,off", MANY)
+def test_quantize_many_rows(cuda_device, T, K, off, dtype, fmt):
+    """Rows enough for several runs of 256 columns per warp (from 9473 runs on)."""
+    assert T * -(-K // 256) > 148 * 64
+    wide = (gen(T, K + off, seed=K) * torch.exp(gen(T, 1, seed=T))).to(dtype)
+    wide[T // 2, off:off + min(K, 128)] = 0
+    x = wide[:, off:]
+    q, s = fp8.quantize_rows(wide.to(cuda_device)[:, off:], fmt)
+    wq, ws = orc.fp8_rows(x, fmt)
+    if fmt == "ue8m0":
+        assert torch.equal(orc.fp8_scale_values(s.cpu()), ws)
+        same_e4m3(q, wq)
+    else:
+        torch.testing.assert_close(s.double().cpu(), ws, rtol=2.0 ** -24, atol=0)
+        # as in test_quantize_rows
+        same_e4m3(q, wq, 0.0 if dtype != torch.float32 else 2.0 ** -15)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,off", MANY)
+def test_quantize_gated_many_rows(cuda_device, T, K, off, dtype, fmt):
+    wide = (2 * gen(T, 2 * K + off, seed=K)).to(dtype)
+    g, u = wide[:, off:].double().chunk(2, 1)
+    q, s = fp8.quantize_rows(wide.to(cuda_device)[:, off:], fmt, gated=True)
+    wq, ws = orc.fp8_rows(g / (1 + torch.exp(-g)) * u, fmt)
+    if fmt == "ue8m0":
+        assert torch.equal(orc.fp8_scale_values(s.cpu()), ws)
+    else:
+        torch.testing.assert_close(s.double().cpu(), ws, rtol=8 * 2.0 ** -24, atol=0)
+    same_e4m3(q, wq, 2.0 ** -13)  # as in test_quantize_gated
+
+
+def test_gated_scales_of_many_rows_next_to_a_power_of_two(cuda_device):
+    """As test_gated_scale_next_to_a_power_of_two, in each group that a warp holds
+    of rows with several runs."""
+    T, K = 2400, 1024
+    assert T * -(-K // 256) > 148 * 64
+    n = K // 128
+    g = 1 + 3 * torch.rand(T, n, generator=torch.Generator().manual_seed(4))
+    silu = g.double() / (1 + torch.exp(-g.double()))
+    u = (448 * 2.0 ** (torch.arange(T * n).view(T, n) % 12 - 6) / silu).float()
+    x = torch.zeros(T, 2 * K)
+    at = 128 * torch.arange(n) + 5 + 17 * torch.arange(n) % 123
+    x[:, at], x[:, K + at] = g, u
+    act = silu * u.double()
+    up = (act / 448).log2() % 1 < 0.5
+    assert up.any() and not up.all()
+    _, s = fp8.quantize_rows(x.to(cuda_device), "ue8m0", gated=True)
+    want = torch.cat([orc.fp8_rows(act[:, j:j + 1], "ue8m0")[1] for j in range(n)], 1)
+    assert torch.equal(orc.fp8_scale_values(s.cpu()), want)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_quantize_nan_inf_and_extremes(cuda_device, fmt):
     x = gen(6, 256, seed=9)
