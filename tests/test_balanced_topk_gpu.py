@@ -242,6 +242,45 @@ def test_gradient(cuda_device, T, E, k, G, kept, score, renorm):
         assert (err <= room + STEP[dtype] * want.abs() + tiny).all()
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k,G,kept", SHAPES)
+def test_gradient_of_each_entry(cuda_device, T, E, k, G, kept, score, renorm):
+    """Each entry to its own size. An entry is p_e (g_e - m) (times 1 - s_e for the
+    sigmoid) with m = sum_i g_i p_i, p the scores or, renormalised, their shares,
+    g_e = 0 for one not chosen, and no m for sigmoids that are not renormalised.
+    p_e is off by RTOL of itself, m by RTOL sum_i |g_i p_i|; the difference, the
+    products and 1 - s_e (under 8 roundings) fit in as much again."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        logits, bias = inputs(T, E, dtype, 5 * T + E, 0.2 if score == "sigmoid" else 1.0 / E)
+        x = logits.to(cuda_device).requires_grad_()
+        gw = torch.randn(T, k, generator=torch.Generator().manual_seed(3))
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, renormalize=renorm,
+                                  num_expert_group=G, topk_group=kept, scoring_func=score,
+                                  routed_scaling_factor=1.5)
+        w.backward(gw.to(cuda_device))
+        ids = ids.cpu().long()
+        want = formula(logits, bias, gw, k, score, renorm, 1.5, ids)
+        l = logits.double()
+        s = torch.sigmoid(l) if score == "sigmoid" else torch.softmax(l, -1)
+        p = s / s.gather(1, ids).sum(1, keepdim=True) if renorm else s
+        g = torch.zeros(T, E, dtype=torch.float64).scatter_(1, ids, 1.5 * gw.double())
+        chosen = torch.zeros(T, E, dtype=torch.bool).scatter_(1, ids, True)
+        m = (g * p).abs().sum(1, keepdim=True)
+        if score == "sigmoid":
+            p = p * (1 - s)
+            m = m if renorm else torch.zeros_like(m)
+        if renorm or score == "sigmoid":
+            # 0 by the formula for one not chosen; autograd's two terms for it cancel
+            # to 2^-53 of themselves
+            p, want = (torch.where(chosen, v, torch.zeros_like(v)) for v in (p, want))
+        room = 2 * RTOL * p * (g.abs() + m)
+        err = (x.grad.double().cpu() - want).abs()
+        # an fp16 entry below 2^-14 is subnormal: half a step of 2^-24
+        tiny = 2.0 ** -25 * (p > 0) if dtype == torch.float16 else 0.0
+        assert (err <= room + STEP[dtype] * want.abs() + tiny).all()
+
+
 def test_gradient_against_differences(cuda_device):
     """(f(l + h) - f(l - h)) / 2h of the fp64 definition at fixed ids."""
     T, E, k = 3, 24, 4
