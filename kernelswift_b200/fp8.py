@@ -79,8 +79,8 @@ def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, inde
 
 
 def _addend(addend: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, index: int,
-            out: torch.Tensor):
-    """(pointer, row stride) of the addend."""
+            out: torch.Tensor | None):
+    """(pointer, row stride) of the addend; `out` where the caller gave one."""
     _no_grad_needed("addend", addend)
     if addend.shape != (rows, cols) or addend.dtype != dtype or addend.get_device() != index:
         raise ValueError(f"addend must be a {dtype} [{rows}, {cols}] tensor on the operands' "
@@ -88,7 +88,8 @@ def _addend(addend: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, inde
     if addend.numel() and (addend.stride(1) != 1 and cols > 1
                            or addend.stride(0) < cols and rows > 1):
         raise ValueError("addend must have dense rows")
-    _check_apart(out, addend)
+    if out is not None:
+        _check_apart(out, addend)
     return addend.data_ptr(), max(addend.stride(0), cols)
 
 
@@ -98,7 +99,7 @@ def _check_apart(out: torch.Tensor, addend: torch.Tensor) -> None:
     column mean nothing."""
     size, (rows, cols) = out.element_size(), out.shape
     apart = (addend.data_ptr() - out.data_ptr()) // size
-    pitch, add_pitch = (t.stride(0) if rows > 1 else cols for t in (out, addend))
+    pitch, add_pitch = (out.stride(0), addend.stride(0)) if rows > 1 else (cols, cols)
     if not out.numel() or apart == 0 and pitch == add_pitch:
         return
     if apart >= (rows - 1) * pitch + cols or -apart >= (rows - 1) * add_pitch + cols:
@@ -213,16 +214,16 @@ def block_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     if x_scale.shape != (T, kb) or w_scale.shape != (nb, kb):
         raise ValueError(f"scales must be [{T}, {kb}] and [{nb}, {kb}], got "
                          f"{tuple(x_scale.shape)} and {tuple(w_scale.shape)}")
-    if out is None:
-        if out_dtype not in _FLOAT_CODE:
-            raise ValueError("out_dtype must be bf16, f16 or f32")
-        out = torch.empty(T, N, dtype=out_dtype, device=x.device)
-        ld_out = N
-    else:
+    if out is not None:
         out_dtype = out.dtype
         _check_out(out, T, N, out_dtype, index)
-        ld_out = max(out.stride(0), N)
+    elif out_dtype not in _FLOAT_CODE:
+        raise ValueError("out_dtype must be bf16, f16 or f32")
     add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, N, out_dtype, index, out)
+    if out is None:
+        out, ld_out = torch.empty(T, N, dtype=out_dtype, device=x.device), N
+    else:
+        ld_out = max(out.stride(0), N)
     if x_scale.requires_grad or w_scale.requires_grad:
         _no_grad_needed("x_scale", x_scale)
         _no_grad_needed("w_scale", w_scale)
@@ -290,11 +291,11 @@ def swiglu_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: 
         raise ValueError(f"scales must be [{gb}, {hb}] and [{hb}, {ib}], got "
                          f"{tuple(w13_scale.shape)} and {tuple(w2_scale.shape)}")
     x = _rows_of(x)
-    if out is None:
-        out = torch.empty(T, H, dtype=x.dtype, device=x.device)
-    else:
+    if out is not None:
         _check_out(out, T, H, x.dtype, index)
     add_ptr, add_ld = (None, 0) if addend is None else _addend(addend, T, H, x.dtype, index, out)
+    if out is None:
+        out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     code = _DTYPE_CODE[x.dtype]
     # of its own: a workspace kept by stream would be shared by captured graphs
     ws = torch.empty(_mlp_workspace_bytes(T, H, inter, code, fmt), dtype=torch.uint8,
