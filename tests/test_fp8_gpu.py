@@ -361,6 +361,43 @@ def test_operand_layouts(cuda_device, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,N,K", [(5, 130, 700), (200, 264, 1100), (2100, 1290, 700)])
+def test_parts_of_operands(cuda_device, T, N, K, fmt):
+    """Rows and k-blocks of larger operands, scales repeated or transposed, a
+    status word that stays 0."""
+    x, w = operands(T + 3, N, K, fmt, cuda_device, 6)
+    status = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+
+    def run(xq, xs, wq, ws):
+        return fp8.block_matmul(xq, xs, wq, ws, out_dtype=torch.float32, status=status[1:])
+
+    def check(got, xq, xs, wq, ws):
+        want, mag = dense64((xq, xs), (wq, ws))
+        room = 2.0 ** -24 * want.abs() + (4 + K / 32) * 2.0 ** -23 * mag
+        assert ((got.double() - want).abs() <= room).all()
+
+    rows = x[0][2:T + 2], x[1][2:T + 2], *w
+    check(run(*rows), *rows)
+    blocks = x[0][:, 128:], x[1][:, 1:], w[0][:, 128:], w[1][:, 1:]
+    check(run(*blocks), *blocks)
+    one = x[0], x[1][:1].expand(T + 3, -1), w[0], w[1].t().contiguous().t()
+    check(run(*one), *one)
+    assert not status.any()
+
+
+def test_scales_at_the_ends_of_their_range(cuda_device):
+    """Powers of two far from 1 on one side and back on the other."""
+    for T in (7, 40, 300, 2100):
+        x, w = operands(T, 1290, 256, "ue8m0", cuda_device, 8)
+        want = fp8.block_matmul(*x, *w, out_dtype=torch.float32)
+        for up in (-100, -20, 20, 100):
+            xs = (x[1].int() + up).to(torch.uint8)
+            ws = (w[1].int() - up).to(torch.uint8)
+            got = fp8.block_matmul(x[0], xs, w[0], ws, out_dtype=torch.float32)
+            assert torch.equal(got, want), (T, up)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("T", [1, 20, 150])
 def test_nan_and_inf_stay_in_their_rows(cuda_device, T, fmt):
     x0 = gen(T, 300, seed=1)
@@ -555,6 +592,37 @@ def test_swiglu_mlp(cuda_device, T, H, I, fmt):
     assert orc.rel_l2(out.double().cpu(), want) < 2.0 ** -8
     err = (out.double().cpu() - want).abs()
     assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -3 * want.abs().amax()).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,I", [(1, 250, 100), (33, 512, 200), (300, 648, 384)])
+def test_swiglu_mlp_types_and_places(cuda_device, T, H, I, dtype, fmt):
+    """Each type, with no addend, rows of a wider tensor, the result in place of
+    the input, of the addend, or beside it."""
+    wide = gen(T, H + 5, seed=1, dtype=dtype).to(cuda_device)
+    x = wide[:, 3:H + 3]
+    w13 = fp8.quantize_blocks(gen(2 * I, H, seed=3).to(cuda_device) / H ** 0.5, fmt)
+    w2 = fp8.quantize_blocks(gen(H, I, seed=4).to(cuda_device) / I ** 0.5, fmt)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    out = fp8.swiglu_mlp(x, *w13, *w2, status=status)
+    want = mlp_reference(x.cpu(), w13, w2, fmt, torch.zeros(T, H))
+    assert out.dtype == dtype and not status.any()
+    assert orc.rel_l2(out.double().cpu(), want) < 2.0 ** -8  # as in test_swiglu_mlp
+    add = gen(T, H, seed=2, dtype=dtype).to(cuda_device)
+    added = fp8.swiglu_mlp(x, *w13, *w2, addend=add)
+    assert orc.rel_l2(added.double().cpu(), want + add.double().cpu()) < 2.0 ** -8
+    got = fp8.swiglu_mlp(x, *w13, *w2, addend=add, out=add)
+    assert got is add and torch.equal(got, added)
+    both = fp8.swiglu_mlp(x, *w13, *w2, addend=x)
+    buf = wide.clone()
+    place = buf[:, 3:H + 3]
+    assert torch.equal(fp8.swiglu_mlp(place, *w13, *w2, addend=place, out=place), both)
+    assert torch.equal(buf[:, :3], wide[:, :3]) and torch.equal(buf[:, H + 3:], wide[:, H + 3:])
+    buf = wide.clone()
+    assert torch.equal(fp8.swiglu_mlp(buf[:, 3:H + 3], *w13, *w2, out=buf[:, 3:H + 3]), out)
+    none = fp8.swiglu_mlp(x[:0], *w13, *w2, addend=x[:0])
+    assert none.shape == (0, H) and none.dtype == dtype
 
 
 def test_layer_of_routed_and_shared_experts(cuda_device):
