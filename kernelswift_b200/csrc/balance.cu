@@ -194,12 +194,14 @@ __device__ __forceinline__ void top_two(double v, double& a, double& b) {
 
 // Bit g * lanes_per_group: group g is kept. Groups are compared by half their
 // value, which stays in range where two of the type's lowest numbers are added.
-// err(m) bounds the error of half a value whose terms' halves have magnitudes that
-// add up to m: the terms may cancel, and their roundings do not. Sets `close` when
-// the bounds of a group left out and of the last one kept meet.
-template <typename R, int PL, typename Err>
+// In 32 bits half a value is off by `slack` for its scores, and by 2^-22 of its
+// terms' (halved) magnitudes, which may cancel while their roundings do not: half
+// an ulp of each, lost when its bias was added, as much at most for their sum, and
+// twice that. Sets `close` when a group left out may lie above any of those kept:
+// each has a bound of its own, so the one in doubt need not be the last one kept.
+template <typename R, int PL>
 __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R (&c)[PL],
-                                                int lane, R* scratch, Err err, bool& close) {
+                                                int lane, R* scratch, float slack, bool& close) {
   const int per = p.lanes_per_group;
   const int g = lane >> p.group_shift, sub = lane & (per - 1);
   R a = R(-INFINITY), b = R(-INFINITY);  // the two largest, a >= b
@@ -239,12 +241,13 @@ __device__ __forceinline__ uint32_t kept_groups(const BalanceParams& p, const R 
   }
   const bool mine = g < p.G && sub == 0;
   const bool keep = mine && rank < p.kept;
-  // infinite values are exact: their bounds are NaN or on the far side
-  const R e = err(fabs(ha) + fabs(hb));
-  const R last =
-      __shfl_sync(0xffffffffu, value - e,
-                  __ffs(__ballot_sync(0xffffffffu, mine && rank == p.kept - 1)) - 1);
-  close = mine && !keep && value + e >= last;
+  if constexpr (std::is_same<R, float>::value) {
+    // infinite values are exact. An infinite kept one's lower bound is NaN, whose key
+    // is above all others, or -inf; one left out has a NaN for its upper bound then
+    const float e = slack + 0x1p-22f * (fabsf(ha) + fabsf(hb));
+    const uint32_t low = __reduce_min_sync(0xffffffffu, keep ? order_key(value - e) : UINT32_MAX);
+    close = mine && !keep && value + e >= key_value(low);
+  }
   return __ballot_sync(0xffffffffu, keep);
 }
 // Bit j: this lane's expert j exists and its group is kept.
@@ -312,7 +315,7 @@ __device__ __noinline__ uint32_t kept_exact(const BalanceParams& p, const Tin* r
   double c[PL];
   exact_scores<PL>(p, row, mx, lane, c);
   bool close = false;
-  return kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
+  return kept_groups(p, c, lane, scratch, 0.0f, close);
 }
 
 // The row's experts in 64 bits, groups included: lane s < k returns the s-th.
@@ -323,7 +326,7 @@ __device__ __noinline__ int select_exact(const BalanceParams& p, const Tin* row,
   exact_scores<PL>(p, row, mx, lane, c);
   uint32_t kept = 0xffffffffu;
   bool close = false;
-  if (p.G > 1) kept = kept_groups(p, c, lane, scratch, [](double) { return 0.0; }, close);
+  if (p.G > 1) kept = kept_groups(p, c, lane, scratch, 0.0f, close);
   uint32_t open = open_experts<PL>(p, kept, lane);
   int sel = 0;
   for (int s = 0; s < p.k; ++s) {
@@ -376,12 +379,9 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   auto tol = [&](float v) { return scores + 2.0f * 2.0f * (PL + 0.5f) * 0x1p-23f * fabsf(v); };
   uint32_t kept = 0xffffffffu;
   if (p.G > 1) {
-    // half a value is off by the error of one score, half an ulp of each (halved)
-    // term, lost when its bias was added, and as much at most for their sum; twice that
+    // half a value has the error of one score
     bool close = false;
-    kept = kept_groups(
-        p, c, lane, reinterpret_cast<float*>(scratch),
-        [&](float m) { return 0.5f * scores + 2.0f * 2.0f * 0x1p-24f * m; }, close);
+    kept = kept_groups(p, c, lane, reinterpret_cast<float*>(scratch), 0.5f * scores, close);
     if (__any_sync(0xffffffffu, close)) kept = kept_exact<PL>(p, row, mx, lane, scratch);
   }
   constexpr uint32_t kLow = PL - 1;

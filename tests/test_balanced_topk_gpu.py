@@ -137,6 +137,26 @@ def test_groups_of_opposite_biases(cuda_device, G, per, kept, score):
         check(logits, bias, w, ids, k, **kw)
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("G,per,kept", [(8, 2, 4), (32, 2, 12), (16, 3, 6)])
+def test_groups_of_opposite_biases_among_others(cuda_device, G, per, kept, score):
+    """Some groups' values are in doubt, their neighbours' in the order are not:
+    a kept one in doubt need not be the last one kept."""
+    T, k = 2048, 6
+    for size, mean in ((1e3, 0), (1e4, 0), (117894.359375, 2), (0.25, -16), (8.0, -12)):
+        g = torch.Generator().manual_seed(int(size) + G)
+        logits = torch.randn(T, G * per, generator=g) * 0.05 + mean
+        bias = size * torch.randint(-2, 3, (G, per), generator=g) / 2
+        pinned = torch.arange(G) % 3 == 0
+        bias[pinned, 0], bias[pinned, 1:] = size, -size
+        bias[torch.arange(G) % 3 == 1] = 0
+        bias = bias.reshape(-1)
+        x = logits.to(cuda_device)
+        kw = dict(num_expert_group=G, topk_group=kept, scoring_func=score)
+        w, ids = fm.balanced_topk(x, x, bias.to(cuda_device), k, **kw)
+        check(logits, bias, w, ids, k, **kw)
+
+
 @pytest.mark.parametrize("G,kept", [(1, 1), (8, 3), (5, 2)])
 def test_biases_of_the_lowest_value(cuda_device, G, kept):
     """Experts masked by the lowest value of fp32 or bf16, of which groups have
