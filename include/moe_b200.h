@@ -537,10 +537,11 @@ int moe_fp8_quantize_blocks(const void* w, int w_dtype, int64_t rows, int64_t co
  * x [num_rows, inner] and w [out_cols, inner] e4m3; x_scale addressed by its
  * two strides, w_scale dense [ceil(out_cols / 128), ceil(inner / 128)];
  * addend (may be NULL) and out in out_dtype (F32/F16/BF16), out may be the
- * addend and shares no element with it otherwise. Products run on the tensor cores and are summed in fp32; with fp32
- * scales each 128-wide block's product is scaled and added in fp32 registers,
- * with UE8M0 the tensor core scales. A row's result does not depend on the
- * other rows' values. `status` as for moe_fused_experts (may be NULL).
+ * addend and shares no element with it otherwise. Products run on the tensor
+ * cores and are summed in fp32; with fp32 scales each 128-wide block's product
+ * is scaled and added in fp32 registers, with UE8M0 the tensor core scales. A
+ * row's result does not depend on the other rows' values. `status` as for
+ * moe_fused_experts (may be NULL).
  */
 int moe_fp8_matmul(const void* x, int64_t ld_x, const void* x_scale, int64_t xs_row_stride,
                    int64_t xs_block_stride, const void* w, int64_t ld_w, const void* w_scale,

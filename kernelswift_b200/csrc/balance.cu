@@ -21,8 +21,8 @@
 // reduced among them; other groups' from shared memory, by 32 / G lanes per group
 // at once (8192 x 256 in 8 groups 13.7 us the first way, 15.3 the second, with lane
 // l holding experts l, l + 32, ...). What bounds it: instruction issue and
-// latency, not its T*E*4 bytes (about 1150 instructions per token of 256 experts
-// in 8 groups). One B200: 8192 x 256 in 8 groups, top 8, 13.7 us; 4096 x 128 6.9
+// latency, not its T*E*4 bytes (about 1090 instructions per token of 256 experts
+// in 8 groups). One B200: 8192 x 256 in 8 groups, top 8, 13.5 us; 4096 x 128 7.3
 // us; 16384 x 384 35 us; one token of 256 3.4 us.
 #include <atomic>
 #include <type_traits>
@@ -452,9 +452,10 @@ __device__ __forceinline__ int select_row(const BalanceParams& p, const Tin* row
   return sel;
 }
 
-// 64 registers for up to 256 experts (8192 x 256 15.4 us against 16.3 with 80). The
+// 64 registers for up to 256 experts (8192 x 256 13.4 us against 14.0 with 80). The
 // parameters stay in constant memory, where the functions out of line read them
-// too (a copy in each thread's local memory cost 1.3 us there).
+// too (with a copy in each thread's local memory 8192 x 256 takes 14.1 us, 16384 x
+// 384 38.5 instead of 34.8).
 template <int PL, typename Tin>
 __global__ void __launch_bounds__(32 * kWarps, PL <= 8 ? 8 : 4)
     balanced_topk_kernel(const __grid_constant__ BalanceParams p) {
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, PL <= 8 ? 8 : 4)
 //   softmax:               dl_e = s_e (g_e - sum_i g_i s_i), g_e = 0 elsewhere
 // One warp per token: it fills the row, then lane j < k stores expert j's
 // entry. Bound by the T*E*b bytes it writes (and reads, for the last form); at
-// 4096 x 128 bf16 it takes 3.2 us (4.7 us in the last form), a fraction of what the
+// 4096 x 128 bf16 it takes 3.1 us (4.3 us in the last form), a fraction of what the
 // autograd engine takes to call it.
 // ---------------------------------------------------------------------------
 

@@ -18,8 +18,8 @@
 //   Bound by the stream of weights and, at a few MB of them, by the fixed cost
 //   of a launch (about 3 us of barrier, TMEM and cluster set-up, pipeline fill
 //   and the last tile's way out). One B200, back to back, UE8M0: 1 x 4096 x 7168
-//   8.9 us (3.3 TB/s), 1 x 36864 x 7168 40.5 us (6.5 TB/s), 16 x 7168 x 2048 6.5
-//   us, 128 x 4096 x 7168 13.6 us; fp32 scales 9.0, 41, 6.8 and 15.3 us.
+//   8.8 us (3.3 TB/s), 1 x 36864 x 7168 40.6 us (6.5 TB/s), 16 x 7168 x 2048 6.6
+//   us, 128 x 4096 x 7168 13.6 us; fp32 scales 8.9, 42, 6.9 and 15.3 us.
 //
 // fp8_pair_kernel: many tokens. Two CTAs share a tile of 256 tokens (lanes) x
 //   256 weight rows (columns), each holding half of either operand; with fp32
@@ -27,11 +27,10 @@
 //   per thread and k-block. Bound by the tensor core at the clock that the power
 //   limit leaves (UE8M0), or by the way of a k-block's product through tensor
 //   memory and registers (fp32 scales). One B200, back to back, UE8M0: 4096 x
-//   4096 x 7168 89 us (2700 TFLOP/s), 16384 x 4096 x 7168 375 to 393 us (by the
-//   clock), 8192 x 7168 x 2048 95 us; fp32 scales 122 us (1970 TFLOP/s), 505 us and
-//   138 us. Tiles of
-//   256 x 256 take an SM's shared memory 512 cycles per k-block for the 512 of its
-//   MMAs; 128 x 256 tiles of single CTAs would take 768.
+//   4096 x 7168 88 us (2740 TFLOP/s), 16384 x 4096 x 7168 369 to 393 us (by the
+//   clock), 8192 x 7168 x 2048 94 us; fp32 scales 122 us (1980 TFLOP/s), 505 us and
+//   139 us. Tiles of 256 x 256 take an SM's shared memory 512 cycles per k-block for
+//   the 512 of its MMAs; 128 x 256 tiles of single CTAs would take 768.
 #include <atomic>
 #include <type_traits>
 
@@ -183,9 +182,11 @@ __device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* tm, int32_t c0
                "r"(c0), "r"(c1)
                : "memory");
 }
-// k-blocks of weights that a CTA asks L2 for while its predecessor still runs: 1 x
-// 4096 x 7168 8.96 us without, 8.58 with 6 (about what fits in the ring), slower
-// again with 16.
+// k-blocks of weights that a CTA asks L2 for while its predecessor still runs, UE8M0
+// and fp32 scales: 1 x 4096 x 7168 9.5 and 9.8 us without, 8.8 and 8.9 with 6 (about
+// what fits in the ring), 8.9 and 9.1 with 16; 16 x 7168 x 2048 6.9 and 7.2, 6.6 and
+// 6.9, 6.6 and 6.9. Of many columns a ring holds fewer k-blocks: 128 x 4096 x 7168
+// 13.2 and 15.5, 13.6 and 15.3, 14.7 and 16.5.
 constexpr int kL2Ahead = 6;
 
 // Asks L2 for the line at `p`.
@@ -292,8 +293,8 @@ struct ColsCfg {
   static constexpr int kGroups = kEpiWarps / 4;       // epilogue groups of 128 lanes
   // A split tile's partials: pushed into the memory of the CTA that sums them
   // where that costs no pipeline stages (BN <= 32), else read from their own
-  // CTA's memory between two cluster barriers (1 x 4096 x 7168 9.7 us read,
-  // 8.6 pushed).
+  // CTA's memory between two cluster barriers (UE8M0, 16 x 4096 x 7168 9.5 us read,
+  // 9.3 pushed; 16 x 7168 x 2048 6.9 and 6.6; 1 x 4096 x 7168 8.95 and 8.75).
   static constexpr bool kPush = BN <= 32;
   static constexpr int kRecvBytes = kPush ? 16384 : 0;
   static constexpr int kOutBytes =  // staged output, or received partials
@@ -1544,10 +1545,11 @@ constexpr PlanCost kCost[2] = {
     {265, 0.3, 170, 0.4, 0, 15, 1100, 28, 275, 3400}};  // UE8M0
 
 // Both sides measured, UE8M0, one B200, back to back: 16 x 4096 x 7168 in 8
-// pieces 9.5 us, in 4 9.3, unsplit 17.4; 128 x 7168 x 2048 in tiles of 32 tokens 8.6 us,
-// of 128 10.0, of 128 in two pieces 12.4; 512 x 4096 x 7168 as pairs 21.8 us, in
-// tiles of 128 22.0; 1024 x 4096 x 7168 25.4 and 38.8. fp32 scales: 512 x 4096 x
-// 7168 as pairs 37.1 us, in tiles of 128 29.2; 1024 x 4096 x 7168 39.2 and 55.4.
+// pieces 9.4 us, in 4 9.5, unsplit 17.4; 128 x 7168 x 2048 in tiles of 32 tokens 8.7 us,
+// of 128 9.2, of 128 in two pieces 13.4; 512 x 4096 x 7168 as pairs 21.9 us (which
+// the model takes), in tiles of 128 21.4; 1024 x 4096 x 7168 24.5 and 37.6. fp32
+// scales: 512 x 4096 x 7168 as pairs 37.1 us, in tiles of 128 28.8; 1024 x 4096 x
+// 7168 38.8 and 55.2.
 // In 32 bits, which check_sizes allows, and by shifts: a call makes a plan.
 Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
   const uint32_t tokens = uint32_t(T), blocks = uint32_t(ceil_div(N, kLanes));
@@ -1561,7 +1563,7 @@ Plan plan_matmul(int64_t T, int64_t N, int64_t K, bool mx, int sms) {
     const uint32_t tiles = ((tokens + bn - 1) >> lb) * blocks;
     const uint32_t occ = bn <= 64 ? 2 : 1;
     // clusters of other sizes leave SMs idle: 16 x 7168 x 18432 in 4 pieces
-    // 24.3 us, in 5 28.6
+    // 24.5 us, in 5 29.0
     for (int ls = 0; ls <= 3 && (1u << ls) <= kbs; ++ls) {
       const uint32_t ctas = tiles << ls;
       if (ls > 0 && ctas > all * occ) break;

@@ -2,9 +2,10 @@
 // on one workspace (quantise, gate-up product, silu(gate) * up quantised, down
 // product with the addend in its epilogue). What bounds it: at a few tokens
 // the stream of 3 H I weight bytes plus the launches, at many tokens the two
-// products. One B200, 7168 x 2048, back to back: 16 tokens 22.8 us (44 MB
-// of weights), 2048 tokens 89 us (UE8M0, 2030 TFLOP/s) and 114 us (fp32 scales);
-// with an addend 91 and 125 us.
+// products. One B200, 7168 x 2048, back to back, UE8M0 and fp32 scales: 1 token 21.0
+// and 21.3 us, 16 tokens 21.8 and 22.5 us (44 MB of weights), 64 tokens 24.2 and 26.5
+// us, 2048 tokens 87 us (2070 TFLOP/s) and 114 us; with an addend 16 tokens take 22.2
+// and 22.9 us, 2048 tokens 92 and 127 us.
 #include "common.cuh"
 
 namespace ksw {
