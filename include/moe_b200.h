@@ -518,8 +518,10 @@ int moe_balanced_topk_backward(const void* router_logits, int logits_dtype, cons
  * all-zero group), q = the e4m3 nearest to x * 448 / absmax. UE8M0: the least
  * power of two with absmax / scale <= 448, q nearest to x / scale. A NaN stays
  * a NaN and does not count for absmax; a group that holds an infinity has an
- * infinite scale (fp32), or saturates there (UE8M0). The scale of row t,
- * block kb goes to scale[t * scale_row_stride + kb * scale_block_stride].
+ * infinite scale (fp32), or saturates there (UE8M0). silu is computed in fp32:
+ * below a gate of -87 its exponential is under the normal range and loses
+ * digits, below -104 it is 0. The scale of row t, block kb goes to
+ * scale[t * scale_row_stride + kb * scale_block_stride].
  */
 int moe_fp8_quantize_rows(const void* x, int x_dtype, int64_t num_rows, int64_t cols,
                           int64_t ld_x, int gated, int scale_format, void* q, int64_t ld_q,

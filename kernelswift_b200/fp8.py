@@ -10,9 +10,10 @@ formats per expert.
 
 Everything runs in libmoe_b200.so on the current stream of the operands'
 device; nothing allocates but the outputs, and a call can be captured in a
-CUDA graph. There is no CPU path and no gradient: these are serving operators,
-which refuse operands that need one or carry a tangent (quantize_blocks takes
-weights that need a gradient as they are).
+CUDA graph. There is no CPU path and no gradient: these are serving operators.
+Activations, scales, addends and outputs that need one are refused (e4m3 operands
+and the weights of quantize_blocks are taken as constants), and so is anything that
+carries a tangent.
 """
 from __future__ import annotations
 
